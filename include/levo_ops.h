@@ -56,7 +56,8 @@ typedef enum {
     /* SnakeBeta parameters already prepared by levo_snake_params_prepare():
      * the alpha pointer holds alpha = exp(alpha_log) and the beta pointer holds
      * 1/beta = 1/(exp(beta_log) + 1e-9), both F32; a bias given with it is F32. */
-    LEVO_DTYPE_SNAKE_PREPARED = 2
+    LEVO_DTYPE_SNAKE_PREPARED = 2,
+    LEVO_DTYPE_BF16 = 3 /* rotary positions and sampling only */
 } levo_dtype;
 
 LEVO_OPS_API uint32_t levo_ops_abi_version(void);
@@ -610,6 +611,156 @@ LEVO_OPS_API int levo_greedy_tokens_f32(const float *logits, int64_t rows, int64
                                         const int64_t *recent, int64_t recent_len, float penalty,
                                         int64_t penalty_limit, const int64_t *ignore, int64_t n_ignore,
                                         int64_t *tokens_out, int32_t *status, levo_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* rotary positions on q and k                                                */
+/* ------------------------------------------------------------------------- */
+/*
+ * Pair i < rotary_dim / 2 of a head at position p turns by phi = p * theta[i]:
+ *   y1 = magnitude * (x1 cos(phi) - x2 sin(phi))
+ *   y2 = magnitude * (x1 sin(phi) + x2 cos(phi))
+ * with (x1, x2) = (x[i], x[i + rotary_dim/2]), or (x[2i], x[2i+1]) with
+ * LEVO_ROPE_INTERLEAVED.  Values from rotary_dim on are copied.
+ * LEVO_ROPE_ADJOINT turns by -phi (same magnitude): the transposed map, which
+ * takes the gradient of an output to the gradient of its input.
+ *
+ * The phase is formed and reduced to a fraction of a turn in 64 bits (its error is
+ * 2^-52 of p * theta, 2e-10 radians at 1e6; |p * theta| < 2^50 is required), so far
+ * positions turn as exactly as near ones.  Sine, cosine, products and sums are F32,
+ * rounded once to the tensor's type (F32, F16 or BF16).
+ */
+#define LEVO_ROPE_INTERLEAVED 1u
+#define LEVO_ROPE_ADJOINT 2u
+
+/* [batch][tokens][heads][head_dim]: any layout with unit stride in head_dim. */
+typedef struct {
+    const void *in;
+    void *out;             /* may be `in` with the same strides (in place) */
+    int64_t heads;         /* 0: no such tensor, its pointers are ignored */
+    int64_t in_stride[3];  /* elements between batches, tokens, heads; 0 (broadcast) is allowed */
+    int64_t out_stride[3]; /* the same for `out`, whose elements must be distinct */
+} levo_rope_tensor;
+
+typedef struct {
+    levo_rope_tensor q, k;
+    int64_t batch, tokens;
+    int64_t head_dim, rotary_dim; /* rotary_dim even, 2..head_dim */
+    const double *theta;          /* device F64 [rotary_dim/2]: radians a position */
+    const int64_t *positions;     /* device [batch][tokens] by position_stride; NULL: start + token */
+    int64_t position_stride[2];   /* elements between batches, tokens; 0 is allowed */
+    int64_t start;
+    int32_t dtype;                /* LEVO_DTYPE_F32, _F16 or _BF16: all tensors of the call */
+    uint32_t flags;
+    float magnitude;              /* 1, or the attention scale of a long-context scheme */
+} levo_rope;
+
+LEVO_OPS_API int levo_rope_qk(const levo_rope *rope, levo_stream_t stream);
+
+/*
+ * theta of the usual schemes, written to HOST memory [rotary_dim/2]:
+ *   theta[i] = base^(-2i/rotary_dim)
+ *   LEVO_ROPE_SCALE_LINEAR    theta[i] / factor
+ *   LEVO_ROPE_SCALE_NTK       base is taken as base * factor^(rotary_dim/(rotary_dim-2))
+ *   LEVO_ROPE_SCALE_BY_PARTS  r = context * theta[i] / 2pi turns over the trained context,
+ *                             g = clamp((r - slow) / (fast - slow), 0, 1),
+ *                             (1 - g) theta[i] / factor + g theta[i]
+ * factor >= 1; context, slow and fast matter to BY_PARTS alone (context > 0, 0 <= slow < fast).
+ */
+typedef enum {
+    LEVO_ROPE_SCALE_NONE = 0,
+    LEVO_ROPE_SCALE_LINEAR = 1,
+    LEVO_ROPE_SCALE_NTK = 2,
+    LEVO_ROPE_SCALE_BY_PARTS = 3
+} levo_rope_scaling;
+
+LEVO_OPS_API int levo_rope_theta_host(double *theta_host, int64_t rotary_dim, double base, int32_t scaling,
+                                      double factor, double context, double slow, double fast);
+
+/*
+ * A token step's rotary positions with the append to the KV cache, in one launch.
+ * Token s of sequence b belongs to cache row lengths[b] + s:
+ *   k.out[b][lengths[b] + s] = k turned, v.out[b][lengths[b] + s] = v    for s < counts[b],
+ *   q.out[b][s]              = q turned                                  for every s.
+ * The caches are [batch][capacity][heads][dim] by k.out_stride / v.out_stride; every other
+ * row of theirs is left as it was.  Positions default to lengths[b] + s (+ rope.start).
+ * lengths and counts lie on the device, so a captured graph serves every step: the caller
+ * advances them.  A sequence's lengths are the same for all layers of a step and are not written.
+ * rope.flags may not hold LEVO_ROPE_ADJOINT.
+ * status (optional device int32, zeroed by the caller): LEVO_APPEND_NO_ROOM when a row would
+ * lie outside [0, capacity) (it is not written), LEVO_APPEND_BAD_COUNT when a count lies outside
+ * [0, tokens] (taken as the nearer end).
+ */
+#define LEVO_APPEND_NO_ROOM 1
+#define LEVO_APPEND_BAD_COUNT 2
+
+typedef struct {
+    levo_rope rope;          /* q as for levo_rope_qk; k.out is the K cache */
+    levo_rope_tensor v;      /* v.out is the V cache */
+    int64_t v_dim;           /* values of a v head */
+    int64_t capacity;        /* rows of a sequence in both caches */
+    const int64_t *lengths;  /* device [batch]: rows held before the call */
+    const int64_t *counts;   /* device [batch]: tokens that are real; NULL: all */
+    int32_t *status;
+} levo_rope_append;
+
+LEVO_OPS_API int levo_rope_append_kv(const levo_rope_append *append, levo_stream_t stream);
+
+/* ------------------------------------------------------------------------- */
+/* next-token sampling: temperature, top-k, top-p, min-p                      */
+/* ------------------------------------------------------------------------- */
+/*
+ * For each row of logits (F32, F16 or BF16, row stride ld), from one given uniform number:
+ *   1. the repetition penalty and the ignore list of levo_greedy_tokens_f32 (the logit taken as
+ *      F32, the division rounded to F32); the list holds for rows r with r % streams == 0
+ *      (streams = token streams of a song; 0: row 0 alone, as there);
+ *   2. the order: larger logit first, equal logits by index; m the first logit,
+ *      w_j = exp((l_j - m) / temperature); temperature 0 takes the first token with probability 1;
+ *   3. top_k: the first k of the order (0: all);
+ *      top_p: of these, token j stays if the weight before it is below top_p of their whole weight
+ *             (1: all; the first always stays);
+ *      min_p: of these, token j stays if w_j >= min_p (0: all; the first always stays);
+ *   4. tokens_out[row] = the first token in the order whose weight together with that of the
+ *      tokens before it exceeds uniforms[row] of the weight of what stayed;
+ *      logprob_out[row] (optional) = log of its share of that weight.
+ * Weights are evaluated in F64 and summed as integers of 2^-44 (of the first token's weight):
+ * no sum depends on an order, the same input always gives the same token, and a token below
+ * 2^-45 of the first has no weight.  +inf logits share the whole weight; -inf and NaN have none.
+ * The settings hold for every row unless their per-row device array is given.
+ * status (optional device int32, zeroed by the caller), bits:
+ *   LEVO_SAMPLE_NAN    a logit is NaN (taken as -inf);
+ *   LEVO_SAMPLE_EMPTY  a row without a token of weight: tokens_out 0, logprob -inf;
+ *   LEVO_SAMPLE_PARAM  a per-row value outside its range, or a uniform outside [0, 1): a
+ *                      temperature that is negative or not finite counts as 0, a top_p or min_p
+ *                      that is NaN as off, any other as the nearer end of its range.
+ * vocab <= 131072.
+ */
+#define LEVO_SAMPLE_NAN 1
+#define LEVO_SAMPLE_EMPTY 2
+#define LEVO_SAMPLE_PARAM 4
+
+typedef struct {
+    const void *logits;
+    int64_t rows, vocab, ld;
+    const float *uniforms;         /* device [rows], in [0, 1) */
+    const float *temperature_rows; /* device [rows] each, or NULL: the value below */
+    const int64_t *top_k_rows;
+    const float *top_p_rows;
+    const float *min_p_rows;
+    int64_t top_k;
+    const int64_t *recent;         /* device [rows][recent_len], ids < 0 skipped; NULL: no penalty */
+    int64_t recent_len;
+    int64_t penalty_limit;         /* ids in [0, penalty_limit) are penalised; <= 0: vocab */
+    const int64_t *ignore;         /* device [n_ignore] */
+    int64_t n_ignore;
+    int64_t streams;
+    int64_t *tokens_out;
+    float *logprob_out;
+    int32_t *status;
+    float temperature, top_p, min_p, penalty;
+    int32_t dtype;
+} levo_sampling;
+
+LEVO_OPS_API int levo_sample_tokens(const levo_sampling *sampling, levo_stream_t stream);
 
 /* ------------------------------------------------------------------------- */
 /* next (f1)  window assembly: crossfade + crop (+ interleave)                */

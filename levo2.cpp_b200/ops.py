@@ -18,7 +18,7 @@ from typing import Optional
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "liblevo_b200.so"
 
 OK, EINVAL, ELAUNCH, EUNSUPPORTED, ENONFINITE, ECANCELLED, ENOMEM, ECUDA = 0, -1, -2, -3, -4, -5, -6, -7
-DTYPE_F32, DTYPE_F16, DTYPE_SNAKE_PREPARED = 0, 1, 2
+DTYPE_F32, DTYPE_F16, DTYPE_SNAKE_PREPARED, DTYPE_BF16 = 0, 1, 2, 3
 FUSED_TANH = 1
 NORM_F16_BOUNDARY = 1
 CHAIN_TANH, CHAIN_TIMING = 1, 2
@@ -118,6 +118,77 @@ class KernelTiming(ctypes.Structure):
     ]
 
 
+ROPE_INTERLEAVED, ROPE_ADJOINT = 1, 2
+ROPE_SCALINGS = ("none", "linear", "ntk", "by_parts")
+APPEND_NO_ROOM, APPEND_BAD_COUNT = 1, 2
+SAMPLE_NAN, SAMPLE_EMPTY, SAMPLE_PARAM = 1, 2, 4
+
+
+class RopeTensor(ctypes.Structure):
+    _fields_ = [("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("heads", ctypes.c_int64)] + [
+        (f"{side}_stride_{axis}", ctypes.c_int64) for side in ("in", "out") for axis in ("batch", "token", "head")]
+
+
+class Rope(ctypes.Structure):
+    _fields_ = [
+        ("q", RopeTensor),
+        ("k", RopeTensor),
+        ("batch", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("rotary_dim", ctypes.c_int64),
+        ("theta", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("position_stride_batch", ctypes.c_int64),
+        ("position_stride_token", ctypes.c_int64),
+        ("start", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("flags", ctypes.c_uint32),
+        ("magnitude", ctypes.c_float),
+    ]
+
+
+class RopeAppend(ctypes.Structure):
+    _fields_ = [
+        ("rope", Rope),
+        ("v", RopeTensor),
+        ("v_dim", ctypes.c_int64),
+        ("capacity", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+class Sampling(ctypes.Structure):
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("uniforms", ctypes.c_void_p),
+        ("temperature_rows", ctypes.c_void_p),
+        ("top_k_rows", ctypes.c_void_p),
+        ("top_p_rows", ctypes.c_void_p),
+        ("min_p_rows", ctypes.c_void_p),
+        ("top_k", ctypes.c_int64),
+        ("recent", ctypes.c_void_p),
+        ("recent_len", ctypes.c_int64),
+        ("penalty_limit", ctypes.c_int64),
+        ("ignore", ctypes.c_void_p),
+        ("n_ignore", ctypes.c_int64),
+        ("streams", ctypes.c_int64),
+        ("tokens_out", ctypes.c_void_p),
+        ("logprob_out", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("temperature", ctypes.c_float),
+        ("top_p", ctypes.c_float),
+        ("min_p", ctypes.c_float),
+        ("penalty", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+    ]
+
+
 CONV_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(ConvCall), ctypes.c_void_p)
 VELOCITY_FN = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float,
                                ctypes.c_void_p)
@@ -129,6 +200,7 @@ _I32 = ctypes.c_int32
 _U32 = ctypes.c_uint32
 _F = ctypes.c_float
 _INT = ctypes.c_int
+_D = ctypes.c_double
 
 # name -> (restype, argtypes); every symbol include/levo_ops.h declares.
 SIGNATURES = {
@@ -165,6 +237,10 @@ SIGNATURES = {
     "levo_gated_layernorm_modulate_f32": (_INT, [_P, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _F, _P]),
     "levo_vae_decode_noalloc_f32": (_INT, [ctypes.POINTER(Topology), _P, _P, _I64, _P, CONV_FN, _P, _U32, _P]),
     "levo_greedy_tokens_f32": (_INT, [_P, _I64, _I64, _I64, _P, _I64, _F, _I64, _P, _I64, _P, _P, _P]),
+    "levo_rope_qk": (_INT, [ctypes.POINTER(Rope), _P]),
+    "levo_rope_theta_host": (_INT, [_P, _I64, _D, _I32, _D, _D, _D, _D]),
+    "levo_rope_append_kv": (_INT, [ctypes.POINTER(RopeAppend), _P]),
+    "levo_sample_tokens": (_INT, [ctypes.POINTER(Sampling), _P]),
     "levo_latent_to_vae_f32": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
     "levo_latent_normalize_f32": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
     "levo_assemble_windows_f32": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I32, _P, _P]),
@@ -509,6 +585,186 @@ def greedy_tokens_t(logits, recent=None, penalty=1.0, penalty_limit=0, ignore=No
     check(lib().levo_greedy_tokens_f32(_ptr(logits), rows, vocab, logits.stride(0), _ptr(recent), recent_len, penalty,
                                        penalty_limit, _ptr(ignore), ignore.numel() if ignore is not None else 0,
                                        _ptr(out), _ptr(status), _stream(logits.device)))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# token step: rotary positions, KV append, sampling
+# ---------------------------------------------------------------------------
+
+def _dtype_of(t) -> int:
+    import torch
+
+    code = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}.get(t.dtype)
+    if code is None:
+        raise ValueError("tensors must be float32, float16 or bfloat16")
+    return code
+
+
+def _same_device(device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError("all tensors of a call must lie on one CUDA device")
+
+
+def _launch(call, args, device) -> None:
+    """Calls the library on `device` and its current stream, whatever device is current."""
+    import torch
+
+    if device.type != "cuda":
+        raise ValueError("levo_b200 ops take CUDA tensors")
+    if torch.cuda.current_device() == device.index:
+        check(call(ctypes.byref(args), _stream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(call(ctypes.byref(args), _stream(device)))
+
+
+def rope_theta(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+               context: float = 4096.0, slow: float = 1.0, fast: float = 32.0, device=None):
+    """Radians a position of each rotary pair, F64 [rotary_dim/2] (levo_rope_theta_host), on `device`.
+    scaling: "none", "linear", "ntk" or "by_parts"."""
+    import torch
+
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling must be one of {ROPE_SCALINGS}")
+    theta = torch.empty(max(rotary_dim, 0) // 2, dtype=torch.float64)
+    buf = theta if theta.numel() else torch.empty(1, dtype=torch.float64)
+    check(lib().levo_rope_theta_host(buf.data_ptr(), rotary_dim, base, ROPE_SCALINGS.index(scaling), factor, context,
+                                     slow, fast))
+    return theta if device is None else theta.to(device)
+
+
+def _rope_tensor(name, x, out, batch, tokens):
+    """RopeTensor of x [batch, tokens, heads, dim] and its output (any outer strides, unit stride in dim)."""
+    if x.dim() != 4 or x.shape[0] != batch or x.shape[1] != tokens:
+        raise ValueError(f"{name} must be [batch, tokens, heads, dim], its batch and tokens those of q")
+    if out.dim() != 4 or out.dtype != x.dtype:
+        raise ValueError(f"{name}'s output must be a 4-D tensor of its dtype")
+    xs, os_ = x.stride(), out.stride()
+    if (xs[3] != 1 or os_[3] != 1) and x.shape[3] > 1:
+        raise ValueError(f"{name} must have unit stride in its last dimension")
+    return RopeTensor(x.data_ptr(), out.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], os_[0], os_[1], os_[2])
+
+
+def _rope_args(q, k, theta, positions, start, flags, magnitude, q_tensor, k_tensor):
+    import torch
+
+    if theta.dtype != torch.float64 or theta.dim() != 1 or not theta.is_contiguous():
+        raise ValueError("theta must be a contiguous float64 [rotary_dim/2]")
+    batch, tokens, _, dim = q.shape
+    ps = (0, 0)
+    if positions is not None:
+        if positions.dtype != torch.int64:
+            raise ValueError("positions must be int64")
+        if positions.dim() == 1 and positions.shape[0] == tokens:
+            ps = (0, positions.stride(0))
+        elif positions.dim() == 2 and positions.shape[0] == batch and positions.shape[1] == tokens:
+            ps = positions.stride()
+        else:
+            raise ValueError("positions must be [tokens] or [batch, tokens]")
+    return Rope(q_tensor, k_tensor, batch, tokens, dim, 2 * theta.shape[0], theta.data_ptr(), _ptr(positions), ps[0],
+                ps[1], start, _dtype_of(q), flags, magnitude)
+
+
+def rope_qk_t(q, k, theta, positions=None, *, start=0, interleaved=False, adjoint=False, magnitude=1.0, q_out=None,
+              k_out=None):
+    """Turns q and k [batch, tokens, heads, dim] (k may be None) by their positions; returns (q_out, k_out).
+    theta: rope_theta(...) on the device, its pairs the first 2 * len(theta) values of a head; positions int64
+    [tokens] or [batch, tokens] (default: start + token).  adjoint=True gives the gradients of q and k from those
+    of the outputs.  Any outer strides; an output may be its input."""
+    import torch
+
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    if k is not None:
+        k_out = torch.empty_like(k) if k_out is None else k_out
+        if k.dtype != q.dtype or k.shape[-1] != q.shape[-1]:
+            raise ValueError("q and k must share a dtype and a head dimension")
+        if k_out.shape != k.shape:
+            raise ValueError("k_out must have the shape of k")
+    if q.dim() != 4 or q_out.shape != q.shape:
+        raise ValueError("q must be [batch, tokens, heads, dim] and q_out of its shape")
+    _same_device(q.device, k, theta, positions, q_out, k_out)
+    batch, tokens = q.shape[:2]
+    args = _rope_args(q, k, theta, positions, start,
+                      (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_ADJOINT if adjoint else 0), magnitude,
+                      _rope_tensor("q", q, q_out, batch, tokens),
+                      RopeTensor() if k is None else _rope_tensor("k", k, k_out, batch, tokens))
+    _launch(lib().levo_rope_qk, args, q.device)
+    return q_out, k_out
+
+
+def rope_append_kv_t(q, k, v, theta, k_cache, v_cache, lengths, *, counts=None, positions=None, start=0,
+                     interleaved=False, magnitude=1.0, q_out=None, status=None):
+    """Turns q [batch, tokens, heads, dim] and appends turned k and v to the caches [batch, capacity, kv heads,
+    dim]: token s < counts[b] of sequence b goes to row lengths[b] + s (int64 device tensors, not advanced here).
+    Returns q_out; APPEND_NO_ROOM / APPEND_BAD_COUNT in the optional status word."""
+    import torch
+
+    q_out = torch.empty_like(q) if q_out is None else q_out
+    if q.dim() != 4 or q_out.shape != q.shape:
+        raise ValueError("q must be [batch, tokens, heads, dim] and q_out of its shape")
+    batch, tokens, _, dim = q.shape
+    for name, x, cache in (("k", k, k_cache), ("v", v, v_cache)):
+        if x.dtype != q.dtype:
+            raise ValueError("q, k and v must share a dtype")
+        if cache.dim() != 4 or cache.shape[0] != batch or x.dim() != 4 or cache.shape[2:] != x.shape[2:]:
+            raise ValueError(f"the {name} cache must be [batch, capacity, heads, dim] as {name} is")
+    if k.shape[3] != dim:
+        raise ValueError("q and k must share a head dimension")
+    if k_cache.shape[1] != v_cache.shape[1]:
+        raise ValueError("the caches must share a capacity")
+    for name, t in (("lengths", lengths), ("counts", counts)):
+        if t is not None and (t.dtype != torch.int64 or t.shape != (batch,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int64 [batch]")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor")
+    _same_device(q.device, k, v, theta, k_cache, v_cache, lengths, counts, positions, q_out, status)
+    rope = _rope_args(q, k, theta, positions, start, ROPE_INTERLEAVED if interleaved else 0, magnitude,
+                      _rope_tensor("q", q, q_out, batch, tokens), _rope_tensor("k", k, k_cache, batch, tokens))
+    args = RopeAppend(rope, _rope_tensor("v", v, v_cache, batch, tokens), v.shape[3], k_cache.shape[1],
+                      lengths.data_ptr(), _ptr(counts), _ptr(status))
+    _launch(lib().levo_rope_append_kv, args, q.device)
+    return q_out
+
+
+def sample_tokens_t(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, recent=None, penalty=1.0,
+                    penalty_limit=0, ignore=None, streams=0, logprobs=None, status=None, out=None):
+    """One token per row of logits [rows, vocab] from uniforms [rows] in [0, 1) (levo_sample_tokens); returns the
+    int64 tokens.  temperature, top_p, min_p (float32) and top_k (int64) are numbers or [rows] tensors; logprobs
+    (float32 [rows], optional) receives the log of each token's share; SAMPLE_* bits in the optional status word."""
+    import torch
+
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be [rows, vocab] with unit stride in vocab")
+    rows, vocab = logits.shape
+    out = torch.empty(rows, dtype=torch.int64, device=logits.device) if out is None else out
+    f32, i64 = torch.float32, torch.int64
+    rowwise = [None, None, None, None]
+    scalar = [temperature, top_k, top_p, min_p]
+    for n, (value, dtype, off) in enumerate(((temperature, f32, 1.0), (top_k, i64, 0), (top_p, f32, 1.0),
+                                             (min_p, f32, 0.0))):
+        if isinstance(value, torch.Tensor):
+            rowwise[n], scalar[n] = value, off
+            if value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous():
+                raise ValueError(f"a per-row setting must be a contiguous {dtype} [rows]")
+    for t, dtype in ((uniforms, f32), (out, i64), (logprobs, f32)):
+        if t is not None and (t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous()):
+            raise ValueError("uniforms and logprobs must be contiguous float32 [rows], out a contiguous int64 [rows]")
+    if recent is not None and (recent.dtype != i64 or recent.dim() != 2 or recent.shape[0] != rows
+                               or not recent.is_contiguous()):
+        raise ValueError("recent must be a contiguous int64 [rows, n]")
+    if ignore is not None and (ignore.dtype != i64 or not ignore.is_contiguous()):
+        raise ValueError("ignore must be a contiguous int64 tensor")
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise ValueError("status must be an int32 tensor")
+    _same_device(logits.device, uniforms, *rowwise, recent, ignore, logprobs, status, out)
+    args = Sampling(logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, uniforms.data_ptr(),
+                    _ptr(rowwise[0]), _ptr(rowwise[1]), _ptr(rowwise[2]), _ptr(rowwise[3]), scalar[1], _ptr(recent),
+                    0 if recent is None else recent.shape[1], penalty_limit, _ptr(ignore),
+                    0 if ignore is None else ignore.numel(), streams, out.data_ptr(), _ptr(logprobs), _ptr(status),
+                    scalar[0], scalar[2], scalar[3], penalty, _dtype_of(logits))
+    _launch(lib().levo_sample_tokens, args, logits.device)
     return out
 
 

@@ -1,0 +1,327 @@
+"""Sampling against the 64-bit definition: equal tokens, at the sizes, ties, masks and settings where it can go
+wrong; and the distribution that a grid of uniform numbers draws."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from token_step_reference import DTYPES, logprob_tolerance, penalised, sample_row
+
+pytestmark = pytest.mark.gpu
+VOCAB = 16385  # LeLM codebook 16384 + EOS
+
+
+def run(ops, logits, u, dev, **kw):
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    logprobs = torch.empty(logits.shape[0], device=dev)
+    tokens = ops.sample_tokens_t(logits, u, logprobs=logprobs, status=status, **kw)
+    return tokens.cpu().numpy(), logprobs.cpu().numpy().astype(np.float64), status.item()
+
+
+def check(ops, dev, logits, u, expect_status=0, **kw):
+    """Tokens equal to the definition's and logprobs within the rounding of the weights."""
+    tokens, logprobs, status = run(ops, logits, u, dev, **kw)
+    assert status == expect_status
+    rows, vocab = logits.shape
+    x = penalised(logits, None if kw.get("recent") is None else kw["recent"].cpu().numpy(), kw.get("penalty", 1.0),
+                  kw.get("penalty_limit", 0), None if kw.get("ignore") is None else kw["ignore"].cpu().numpy(),
+                  kw.get("streams", 0))
+
+    def each(name, off):
+        v = kw.get(name, off)
+        return v.cpu().tolist() if isinstance(v, torch.Tensor) else [float(np.float32(v))] * rows
+
+    settings = zip(each("temperature", 1.0), [int(k) for k in each("top_k", 0)], each("top_p", 1.0),
+                   each("min_p", 0.0), u.cpu().tolist())
+    for r, (temperature, top_k, top_p, min_p, uniform) in enumerate(settings):
+        want = sample_row(x[r], uniform, temperature, top_k, top_p, min_p)
+        if want is None:
+            assert tokens[r] == 0 and logprobs[r] == -np.inf
+            continue
+        token, logprob, weight, total, near = want
+        assert tokens[r] == token, f"row {r}: {tokens[r]}, not {token} ({near:.3g} from a border)"
+        tol = logprob_tolerance(logprob, weight, total, vocab)
+        assert abs(logprobs[r] - logprob) <= tol, f"row {r}: logprob {logprobs[r]} not {logprob} +- {tol}"
+    return tokens
+
+
+def uniforms(gen, rows):
+    return torch.rand(rows, generator=gen, device=gen.device)
+
+
+FILTERS = {
+    "none": {}, "k1": {"top_k": 1}, "k50": {"top_k": 50}, "k1500": {"top_k": 1500}, "k over": {"top_k": 10 ** 9},
+    "p0": {"top_p": 0.0}, "p50": {"top_p": 0.5}, "p999": {"top_p": 0.999}, "m0.1": {"min_p": 0.1}, "m1": {"min_p": 1.0},
+    "k+p": {"top_k": 200, "top_p": 0.9}, "all": {"top_k": 300, "top_p": 0.95, "min_p": 0.01, "temperature": 0.7},
+    "hot": {"temperature": 20.0, "top_p": 0.9}, "cold": {"temperature": 0.01}, "zero": {"temperature": 0.0},
+    "k+m": {"top_k": 40, "min_p": 0.05},
+}
+
+
+@pytest.mark.parametrize("name", FILTERS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [1, 2, 31, 33, 1000, VOCAB, 50257])
+def test_sample_matches_definition(ops, dev, dtype, vocab, name):
+    gen = torch.Generator(device=dev).manual_seed(vocab + len(name))
+    logits = (3.0 * torch.randn((5, vocab), generator=gen, device=dev)).to(DTYPES[dtype])
+    check(ops, dev, logits, uniforms(gen, 5), **FILTERS[name])
+
+
+@pytest.mark.parametrize("vocab,rows", [(131072, 1), (131071, 3), (100003, 9), (65536, 2)])
+@pytest.mark.parametrize("name", ["none", "k50", "k1500", "p999", "all", "hot", "m0.1"])
+def test_sample_large_vocabularies(ops, dev, vocab, rows, name):
+    gen = torch.Generator(device=dev).manual_seed(vocab + rows)
+    logits = (2.0 * torch.randn((rows, vocab), generator=gen, device=dev)).bfloat16()
+    check(ops, dev, logits, uniforms(gen, rows), **FILTERS[name])
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 149, 600])
+def test_sample_row_counts(ops, dev, rows):
+    gen = torch.Generator(device=dev).manual_seed(rows)
+    logits = 2.5 * torch.randn((rows, 2000), generator=gen, device=dev)
+    check(ops, dev, logits, uniforms(gen, rows), top_k=100, top_p=0.9)
+    check(ops, dev, logits, uniforms(gen, rows), top_p=0.9)
+
+
+def test_sample_settings_of_each_row(ops, dev):
+    gen = torch.Generator(device=dev).manual_seed(1)
+    rows = 64
+    logits = (3 * torch.randn((rows, VOCAB), generator=gen, device=dev)).half()
+    temperature = 0.3 + 1.5 * uniforms(gen, rows)
+    temperature[::7] = 0.0
+    top_k = torch.randint(0, 3000, (rows,), generator=gen, device=dev)
+    top_k[::3] = 0
+    top_p = uniforms(gen, rows)
+    top_p[::4] = 1.0
+    min_p = 0.2 * uniforms(gen, rows)
+    min_p[::2] = 0.0
+    check(ops, dev, logits, uniforms(gen, rows), temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["none", "k50", "k1500", "p50", "all"])
+def test_sample_ties(ops, dev, dtype, name):
+    """Equal logits are taken by index, inside and at the border of every filter."""
+    gen = torch.Generator(device=dev).manual_seed(2)
+    rows = 12
+    few = torch.randint(0, 9, (rows, VOCAB), generator=gen, device=dev).to(DTYPES[dtype])
+    few[0] = 1.5                                  # all equal
+    few[1] = 0.0
+    few[1, ::2] = -0.0                            # zeros of both signs are equal
+    few[2] = torch.where(torch.arange(VOCAB, device=dev) % 1000 == 7, 5.0, 0.0).to(few.dtype)
+    few[3, 100:] = -math.inf
+    check(ops, dev, few, uniforms(gen, rows), **FILTERS[name])
+
+
+@pytest.mark.parametrize("name", ["none", "k50", "k1500", "p50", "p999", "all", "m0.1"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_masked_rows(ops, dev, dtype, name):
+    """-inf, the type's lowest value, +inf, one token left, none left, a wide range of magnitudes."""
+    gen = torch.Generator(device=dev).manual_seed(3)
+    t, vocab = DTYPES[dtype], 5000
+    x = (3 * torch.randn((9, vocab), generator=gen, device=dev)).to(t)
+    x[0, 1:] = -math.inf
+    x[1, :-1] = torch.finfo(t).min
+    x[2, ::3] = -math.inf
+    x[3, torch.arange(vocab, device=dev) % 50 != 3] = torch.finfo(t).min
+    x[4] = torch.finfo(t).min
+    x[5, [10, 3000, 77]] = math.inf
+    x[6] = -math.inf
+    x[7] = (x[7].float() * 1e4).clamp(-6e4, 6e4).to(t)
+    x[8] = (x[8].float() * 1e-6).to(t)
+    check(ops, dev, x, uniforms(gen, 9), expect_status=ops.SAMPLE_EMPTY, **FILTERS[name])
+
+
+def test_sample_clusters_of_close_logits(ops, dev):
+    """Thousands of different logits within few units of the last place, beside wide ones: no bin splits them at once."""
+    gen = torch.Generator(device=dev).manual_seed(4)
+    vocab = 20000
+    base = torch.full((6, vocab), 7.0, device=dev)
+    base += torch.randint(0, 4000, (6, vocab), generator=gen, device=dev) * 2.0 ** -21
+    base[1, ::2] -= 25.0
+    base[2] *= 1e-30
+    base[3, 0] = 30.0
+    base[4, 5:9000] = -3e38
+    base[5, 7] = 7.5
+    for name in ("none", "k1500", "p50", "k+p", "m0.1"):
+        check(ops, dev, base, uniforms(gen, 6), **FILTERS[name])
+    check(ops, dev, base, uniforms(gen, 6), top_k=9999, top_p=0.7)
+    check(ops, dev, base, uniforms(gen, 6), temperature=1e-6)
+    check(ops, dev, base, uniforms(gen, 6), temperature=1e6, top_p=0.3)
+
+
+def test_sample_nan(ops, dev):
+    x = torch.zeros((3, 100), device=dev)
+    x[1, 42] = math.nan
+    x[2, 5] = math.nan
+    u = torch.full((3,), 0.425, device=dev)
+    tokens, logprobs, status = run(ops, x, u, dev, ignore=torch.tensor([5], device=dev), streams=2)
+    assert status == ops.SAMPLE_NAN                 # row 1's; row 2's NaN is on its ignore list
+    assert tokens.tolist() == [43, 43, 43]          # 99 tokens each; row 0 without 5, row 1 without 42, row 2 without 5
+    assert np.allclose(logprobs, math.log(1 / 99), atol=1e-6)
+    x = torch.full((1, 50), math.nan, device=dev)
+    assert run(ops, x, u[:1], dev)[2] == ops.SAMPLE_NAN | ops.SAMPLE_EMPTY
+
+
+def test_sample_values_out_of_range(ops, dev):
+    """Counted as the header says, and flagged."""
+    rows, vocab = 10, 300
+    gen = torch.Generator(device=dev).manual_seed(5)
+    x = 2 * torch.randn((rows, vocab), generator=gen, device=dev)
+    u = torch.full((rows,), 0.5, device=dev)
+    one = {"temperature": [1.0] * rows, "top_k": [0] * rows, "top_p": [1.0] * rows, "min_p": [0.0] * rows}
+    given = {n: list(v) for n, v in one.items()}
+    taken = {n: list(v) for n, v in one.items()}
+    for r, (n, bad, good) in enumerate((("temperature", -1.0, 0.0), ("temperature", math.nan, 0.0),
+                                        ("temperature", math.inf, 0.0), ("top_k", -3, 0), ("top_p", math.nan, 1.0),
+                                        ("top_p", -0.5, 0.0), ("top_p", 2.0, 1.0), ("min_p", math.nan, 0.0),
+                                        ("min_p", 3.0, 1.0), ("min_p", -1.0, 0.0))):
+        given[n][r], taken[n][r] = bad, good
+
+    def tensors(d):
+        return {n: torch.tensor(v, device=dev, dtype=torch.int64 if n == "top_k" else torch.float32)
+                for n, v in d.items()}
+
+    tokens, logprobs, status = run(ops, x, u, dev, **tensors(given))
+    want, want_lp, clean = run(ops, x, u, dev, **tensors(taken))
+    assert status == ops.SAMPLE_PARAM and clean == 0
+    assert np.array_equal(tokens, want) and np.array_equal(logprobs, want_lp)
+    for r in range(rows):
+        alone = {n: v[r:r + 1] for n, v in tensors(given).items()}
+        assert run(ops, x[r:r + 1], u[r:r + 1], dev, **alone)[2] == ops.SAMPLE_PARAM, r
+    edge = torch.tensor([0.0, 1.0, 7.0, -1.0, math.nan], device=dev)
+    tokens, _, status = run(ops, x[:1].expand(5, vocab).contiguous(), edge, dev, top_k=10)
+    order = torch.sort(x[0], descending=True).indices.tolist()
+    assert status == ops.SAMPLE_PARAM and tokens.tolist() == [order[0], order[9], order[9], order[0], order[0]]
+
+
+def test_sample_penalty_and_ignore_list(ops, dev):
+    gen = torch.Generator(device=dev).manual_seed(6)
+    rows = 12
+    x = 3 * torch.randn((rows, VOCAB), generator=gen, device=dev)
+    recent = torch.randint(-1, VOCAB, (rows, 700), generator=gen, device=dev)
+    recent[:, ::5] = recent[:, 1:2]  # repeats count once
+    top = x.topk(8, dim=1).indices
+    recent[:, 2:10] = top
+    recent[0, 3] = 2 ** 40
+    ignore = torch.cat((top[0, :3], top[3, :2], torch.tensor([-5, VOCAB, 2 ** 33], device=dev)))
+    u = uniforms(gen, rows)
+    for streams in (0, 1, 3):
+        check(ops, dev, x, u, recent=recent, penalty=1.3, penalty_limit=VOCAB - 1, ignore=ignore, streams=streams,
+              top_k=20, top_p=0.9)
+        check(ops, dev, x, u, recent=recent, penalty=0.7, ignore=ignore, streams=streams, top_p=0.95)
+    everything = torch.arange(VOCAB, device=dev)
+    tokens, _, status = run(ops, x, u, dev, ignore=everything, streams=rows)
+    assert tokens[0] == 0 and status == ops.SAMPLE_EMPTY
+
+
+def test_sample_at_temperature_zero_is_the_greedy_choice(ops, dev):
+    gen = torch.Generator(device=dev).manual_seed(7)
+    x = torch.randint(0, 40, (9, VOCAB), generator=gen, device=dev).float()
+    recent = torch.randint(-1, VOCAB, (9, 50), generator=gen, device=dev)
+    ignore = torch.randint(0, VOCAB, (16,), generator=gen, device=dev)
+    kw = {"recent": recent, "penalty": 1.1, "penalty_limit": VOCAB - 1, "ignore": ignore}
+    want = ops.greedy_tokens_t(x, **kw)
+    got = ops.sample_tokens_t(x, uniforms(gen, 9), temperature=0.0, **kw)
+    assert torch.equal(got, want)
+
+
+def test_sample_strided_rows_and_neighbours(ops, dev):
+    gen = torch.Generator(device=dev).manual_seed(8)
+    for t in DTYPES.values():
+        big = (3 * torch.randn((7, 3007), generator=gen, device=dev)).to(t)
+        for lo, hi in ((0, 3000), (1, 2998), (3, 2500)):
+            check(ops, dev, big[:, lo:hi], uniforms(gen, 7), top_p=0.9)
+            check(ops, dev, big[:, lo:hi], uniforms(gen, 7), top_k=64)
+    out = torch.full((9,), -7, dtype=torch.int64, device=dev)
+    lp = torch.full((9,), 5.0, device=dev)
+    ops.sample_tokens_t(big, uniforms(gen, 7), out=out[1:8], logprobs=lp[1:8])
+    assert out[0] == out[8] == -7 and lp[0] == lp[8] == 5.0
+
+
+@pytest.mark.parametrize("kw", [{}, {"top_k": 12}, {"top_p": 0.8}, {"min_p": 0.05}])
+def test_sample_draws_the_distribution(ops, dev, kw):
+    """A grid of n uniform numbers gives each kept token n p rounded down or up, and no other."""
+    gen = torch.Generator(device=dev).manual_seed(9)
+    n, vocab = 20000, 40
+    x = 1.5 * torch.randn((1, vocab), generator=gen, device=dev)
+    u = (torch.arange(n, device=dev) + 0.5) / n
+    tokens = ops.sample_tokens_t(x.expand(n, vocab).contiguous(), u, **kw).cpu().numpy()
+    drawn = np.bincount(tokens, minlength=vocab)
+    row = x[0].cpu().numpy()
+    order = np.argsort(-row, kind="stable")
+    p = np.exp(row[order].astype(np.float64) - row.max())
+    keep = vocab
+    if "top_k" in kw:
+        keep = 12
+    if "top_p" in kw:
+        keep = int(np.sum(np.cumsum(p) - p < np.float32(0.8) * p.sum()))
+    if "min_p" in kw:
+        keep = int(np.sum(p >= np.float32(0.05)))
+    want = np.zeros(vocab)
+    want[order[:keep]] = p[:keep] / p[:keep].sum()
+    assert np.all(np.abs(drawn - n * want) <= 1.0 + 1e-3)  # the grid is F32: 1e-3 of a step off
+    assert np.all(drawn[order[keep:]] == 0)
+
+
+def test_sample_captured_and_replayed_beside_another_graph(ops, dev):
+    gen = torch.Generator(device=dev).manual_seed(10)
+    rows = 4
+    cases = []
+    for vocab, kw in ((VOCAB, {"top_k": 50}), (131072, {"top_p": 0.9}), (VOCAB, {"top_p": 0.95, "min_p": 0.01})):
+        x, u = torch.empty((rows, vocab), device=dev), torch.empty(rows, device=dev)
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+        x.normal_(generator=gen)
+        u.uniform_(generator=gen)
+        ops.sample_tokens_t(x, u, out=out, **kw)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.sample_tokens_t(x, u, out=out, **kw)
+        cases.append((graph, x, u, out, kw))
+    for _ in range(3):
+        for _, x, u, _, _ in cases:
+            x.normal_(generator=gen)
+            u.uniform_(generator=gen)
+        for graph, *_ in cases:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, x, u, out, kw in cases:
+            assert torch.equal(out, ops.sample_tokens_t(x, u, **kw))
+
+
+def test_sample_is_the_same_every_time_and_on_other_streams(ops, dev):
+    gen = torch.Generator(device=dev).manual_seed(11)
+    x = torch.randn((300, VOCAB), generator=gen, device=dev)
+    u = uniforms(gen, 300)
+    lp = torch.empty(300, device=dev)
+    want = ops.sample_tokens_t(x, u, top_p=0.97, logprobs=lp)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=dev) for _ in range(3)]
+    results = []
+    for stream in streams:
+        with torch.cuda.stream(stream):
+            for _ in range(3):
+                again = torch.empty(300, device=dev)
+                results.append((ops.sample_tokens_t(x, u, top_p=0.97, logprobs=again), again))
+    torch.cuda.synchronize()
+    for tokens, again in results:
+        assert torch.equal(tokens, want) and torch.equal(again, lp)
+
+
+def test_sample_on_a_device_that_is_not_current(ops, dev):
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    other = torch.device("cuda:1")
+    gen = torch.Generator(device=dev).manual_seed(12)
+    x, u = torch.randn((3, 1000), generator=gen, device=dev), uniforms(gen, 3)
+    got = ops.sample_tokens_t(x.to(other), u.to(other), top_k=20)
+    assert got.device == other and torch.equal(got.cpu(), ops.sample_tokens_t(x, u, top_k=20).cpu())
+    with pytest.raises(ValueError, match="one CUDA device"):
+        ops.sample_tokens_t(x, u.to(other))
+
+
+def test_sample_no_rows(ops, dev):
+    assert ops.sample_tokens_t(torch.empty((0, 10), device=dev), torch.empty(0, device=dev)).shape == (0,)
