@@ -22,8 +22,6 @@
 namespace levo {
 namespace {
 
-constexpr int kThreads = 256;
-
 // sin and cos of f quarter turns, |f| <= 1/2: f * S(f^2) and C(f^2), the Taylor
 // coefficients (pi/2)^k / k! of the two functions.  The first term left out is
 // (pi/4)^11 / 11! = 1.8e-9 of the sine and (pi/4)^12 / 12! = 1.1e-10 of the cosine.
@@ -34,7 +32,7 @@ constexpr double quarter_coefficient(int k) {
     return c;
 }
 
-struct Turn {
+struct alignas(8) Turn {
     float c, s;
 };
 
@@ -108,60 +106,306 @@ struct RopeArgs {
     int64_t capacity;
     const int64_t *lengths, *counts;
     int32_t *status;
+    // launch shape
+    int turned_chunks, qk_chunks, v_chunks, chunks;  // of q and k that turn, of q and k, of v, the larger
+    uint32_t all_tokens;
+    int lane_chunks, heads_per_block, token_lanes, tile;
 };
 
-// One thread per (token, head, unit): a unit is a pair, or one copied value.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs<T> a) {
-    const int64_t half = a.rotary_dim / 2;
-    const int64_t units_qk = half + (a.head_dim - a.rotary_dim);
-    const int64_t units = units_qk > a.v_dim ? units_qk : a.v_dim;
-    const int64_t heads = a.q.heads + a.k.heads + a.v.heads;
-    const int64_t total = a.batch * a.tokens * heads * units;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int64_t u = i % units;
-        int64_t head = i / units % heads;
-        const int64_t token = i / (units * heads);
-        const int64_t b = token / a.tokens, s = token % a.tokens;
-        const bool is_q = head < a.q.heads;
-        const bool is_v = head >= a.q.heads + a.k.heads;
-        const Side<T> &side = is_q ? a.q : is_v ? a.v : a.k;
-        head -= is_q ? 0 : is_v ? a.q.heads + a.k.heads : a.q.heads;
-        if (u >= (is_v ? a.v_dim : units_qk)) continue;
-        int64_t row = s;
-        int64_t position = a.start + s;
-        if (a.append) {
-            const int64_t at = a.lengths[b] + s;
-            position += at - s;
-            if (!is_q) {
-                const int64_t given = a.counts ? a.counts[b] : a.tokens;
-                if ((given < 0 || given > a.tokens) && a.status) atomicOr(a.status, LEVO_APPEND_BAD_COUNT);
-                if (s >= given) continue;
-                if (at < 0 || at >= a.capacity) {
-                    if (a.status) atomicOr(a.status, LEVO_APPEND_NO_ROOM);
-                    continue;
-                }
-                row = at;
+// VEC neighbouring values: one load or store.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Vec {
+    T v[VEC];
+};
+
+// A head is cut into chunks of two vectors of VEC values, so that a pair never spans threads:
+//   half layout:  vectors c and c + rotary_dim/2/VEC (the two members of VEC pairs);
+//   interleaved:  vectors c and c + n of the 2n (or 2n-1) turned ones, VEC/2 pairs each;
+//   values that are copied (behind rotary_dim, and v): vectors c and c + n of theirs.
+// In every case neighbouring threads touch neighbouring vectors.
+struct Chunk {
+    int first, second;  // offsets in a head; second < 0: none
+};
+
+template <int VEC, bool INTER>
+__device__ __forceinline__ Chunk turned_chunk(int c, int rotary_dim) {
+    if (!INTER) return {c * VEC, rotary_dim / 2 + c * VEC};
+    if (VEC == 1) return {2 * c, 2 * c + 1};
+    const int vectors = rotary_dim / VEC, n = (vectors + 1) / 2;
+    return {c * VEC, c + n < vectors ? (c + n) * VEC : -1};
+}
+
+template <int VEC>
+__device__ __forceinline__ Chunk copied_chunk(int c, int from, int to) {
+    const int vectors = (to - from) / VEC, n = (vectors + 1) / 2;
+    return {from + c * VEC, c + n < vectors ? from + (c + n) * VEC : -1};
+}
+
+// Where pair p's cosine lies (its sine two floats on) among the floats of a token's turns: chunk c's VEC pairs are
+// read as Turns2 c, c + turned_chunks, ... (neighbouring threads on neighbouring ones).
+template <int VEC, bool INTER>
+__device__ __forceinline__ int turn_slot(int p, int turned_chunks) {
+    int c = p / VEC, j = p % VEC;
+    if (INTER && VEC > 1) {
+        constexpr int H = VEC > 1 ? VEC / 2 : 1;
+        const int vector = p / H;
+        const bool late = vector >= turned_chunks;
+        c = late ? vector - turned_chunks : vector;
+        j = p % H + (late ? H : 0);
+    }
+    return 4 * (j / 2 * turned_chunks + c) + j % 2;
+}
+
+// Two values to F32 and back, one instruction each way for the 16-bit types.
+__device__ __forceinline__ float2 to_f32x2(float x, float y) { return make_float2(x, y); }
+__device__ __forceinline__ float2 to_f32x2(__half x, __half y) { return __half22float2(__halves2half2(x, y)); }
+__device__ __forceinline__ float2 to_f32x2(__nv_bfloat16 x, __nv_bfloat16 y) {
+    return __bfloat1622float2(__halves2bfloat162(x, y));
+}
+__device__ __forceinline__ void from_f32x2(float2 v, float &x, float &y) { x = v.x, y = v.y; }
+__device__ __forceinline__ void from_f32x2(float2 v, __half &x, __half &y) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    x = __low2half(h), y = __high2half(h);
+}
+__device__ __forceinline__ void from_f32x2(float2 v, __nv_bfloat16 &x, __nv_bfloat16 &y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    x = __low2bfloat16(h), y = __high2bfloat16(h);
+}
+
+// The turns of two pairs: cosines, then sines.
+struct alignas(16) Turns2 {
+    float2 c, s;
+};
+
+// One pair.  Explicit roundings: every vector width and layout gives the same bits.
+__device__ __forceinline__ float2 turn_pair(float x1, float x2, float c, float s) {
+    return make_float2(__fmaf_rn(x1, c, -__fmul_rn(x2, s)), __fmaf_rn(x1, s, __fmul_rn(x2, c)));
+}
+
+// Turns the VEC pairs that a thread's two vectors hold, two pairs at a time.  turns: the chunk's first Turns2 of the
+// token, the others turned_chunks apart.
+template <typename T, int VEC, bool INTER>
+__device__ __forceinline__ void turn_pairs(Vec<T, VEC> (&x)[2], const Turns2 *turns, int turned_chunks) {
+    if constexpr (VEC == 1) {
+        const Turns2 t = turns[0];
+        const float x1 = to_f32(x[0].v[0]), x2 = to_f32(x[1].v[0]);
+        const float2 y = turn_pair(x1, x2, t.c.x, t.s.x);
+        x[0].v[0] = from_f32<T>(y.x);
+        x[1].v[0] = from_f32<T>(y.y);
+    } else if constexpr (INTER) {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            const Turns2 t = turns[i / 2 * turned_chunks];
+#pragma unroll
+            for (int j = i; j < i + 2; ++j) {
+                T *const pair = &x[j / (VEC / 2)].v[2 * (j % (VEC / 2))];
+                const float2 v = to_f32x2(pair[0], pair[1]);
+                const float c = j > i ? t.c.y : t.c.x, s = j > i ? t.s.y : t.s.x;
+                from_f32x2(turn_pair(v.x, v.y, c, s), pair[0], pair[1]);
             }
         }
-        if (a.positions) position = a.positions[b * a.ps[0] + s * a.ps[1]];
-        const T *in = side.in + b * side.is[0] + s * side.is[1] + head * side.is[2];
-        T *out = side.out + b * side.os[0] + row * side.os[1] + head * side.os[2];
-        if (is_v) {
-            out[u] = in[u];
-        } else if (u >= half) {
-            const int64_t d = a.rotary_dim + (u - half);
-            out[d] = in[d];
-        } else {
-            const int64_t d1 = a.interleaved ? 2 * u : u;
-            const int64_t d2 = a.interleaved ? 2 * u + 1 : u + half;
-            const Turn t = turn_at(static_cast<double>(position), a.theta[u], a.magnitude, a.adjoint != 0);
-            const float x1 = to_f32(in[d1]), x2 = to_f32(in[d2]);
-            out[d1] = from_f32<T>(x1 * t.c - x2 * t.s);
-            out[d2] = from_f32<T>(x1 * t.s + x2 * t.c);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+            const Turns2 t = turns[i / 2 * turned_chunks];
+            const float2 x1 = to_f32x2(x[0].v[i], x[0].v[i + 1]), x2 = to_f32x2(x[1].v[i], x[1].v[i + 1]);
+            const float2 p = __fmul2_rn(x2, t.s);
+            from_f32x2(__ffma2_rn(x1, t.c, make_float2(-p.x, -p.y)), x[0].v[i], x[0].v[i + 1]);
+            from_f32x2(__ffma2_rn(x1, t.s, __fmul2_rn(x2, t.c)), x[1].v[i], x[1].v[i + 1]);
         }
     }
+}
+
+// 384 threads, three CTAs an SM (56 registers): 512 and two, 256 and four were 0 to 10 % slower over the sizes below.
+constexpr int kMaxThreads = 384;
+constexpr int kCtasPerSm = 3;
+// Bytes that a thread has on their way: 128 (four tokens of two 16-byte vectors).  Half and twice that cost 5 % on
+// a 4 x 2048-token prompt: fewer bytes in flight, and fewer, longer CTAs at the end.
+constexpr int kBytesInFlight = 128;
+constexpr int kMaxTurns = 4096;  // of a CTA: 32 KB of shared memory
+constexpr int kMaxTile = 32;     // tokens of a CTA
+
+// A token of the tile: where its values lie (element offsets of the first head of q, k and v; out < 0: k and v have no
+// row in the caches), and its position.
+struct Place {
+    int64_t in[3], out[3];
+    double position;
+};
+
+// One value vector, global to shared memory (asynchronously where the hardware copies that many bytes).
+template <int BYTES>
+__device__ __forceinline__ void copy_in(void *to, const void *from) {
+    if constexpr (BYTES == 16) {
+        cp_async16(to, from);
+    } else if constexpr (BYTES >= 4) {
+        const unsigned dst = static_cast<unsigned>(__cvta_generic_to_shared(to));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(from), "n"(BYTES) : "memory");
+    } else {
+        *static_cast<uint16_t *>(to) = *static_cast<const uint16_t *>(from);
+    }
+}
+
+// A CTA turns a tile of tokens.  A thread keeps one chunk of one head and goes through the tile's tokens: it starts
+// the copies of all its vectors to shared memory (it alone reads them: no registers wait for them and no barrier), the
+// CTA evaluates every sine and cosine of the tile once while they are on their way, and the thread turns and stores.
+template <typename T, int VEC, bool INTER>
+__global__ void __launch_bounds__(kMaxThreads, kCtasPerSm) rope_kernel(const RopeArgs<T> a) {
+    using V = Vec<T, VEC>;
+    constexpr int kPairs2 = (VEC + 1) / 2;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Turns2 *const turns = reinterpret_cast<Turns2 *>(smem);  // [tile token][kPairs2][turned chunk]
+    V *const staged = reinterpret_cast<V *>(smem + a.tile * kPairs2 * a.turned_chunks * sizeof(Turns2));
+    __shared__ Place places[kMaxTile];
+    const uint32_t first_token = blockIdx.x * static_cast<uint32_t>(a.tile);
+    const int tile = static_cast<int>(min(static_cast<uint32_t>(a.tile), a.all_tokens - first_token));
+    const int q_end = static_cast<int>(a.q.heads), k_end = q_end + static_cast<int>(a.k.heads);
+    const int half = static_cast<int>(a.rotary_dim) / 2;
+    // Everything that the sines wait for is loaded first.
+    const double first_theta = a.theta[threadIdx.x % half];
+    int64_t row = 0, position = 0, given = a.tokens;
+    int64_t b = 0, s = 0;
+    if (threadIdx.x < tile) {
+        const uint32_t token = first_token + threadIdx.x;
+        b = token / static_cast<uint32_t>(a.tokens);
+        s = token % static_cast<uint32_t>(a.tokens);
+        if (a.append) row = a.lengths[b];
+        if (a.counts) given = a.counts[b];
+        if (a.positions) position = a.positions[b * a.ps[0] + s * a.ps[1]];
+        Place &p = places[threadIdx.x];
+        p.in[0] = b * a.q.is[0] + s * a.q.is[1];
+        p.in[1] = b * a.k.is[0] + s * a.k.is[1];
+        p.in[2] = b * a.v.is[0] + s * a.v.is[1];
+    }
+    __syncthreads();
+
+    const int lane = static_cast<int>(threadIdx.x) % a.lane_chunks, group = static_cast<int>(threadIdx.x) / a.lane_chunks;
+    const int head = static_cast<int>(blockIdx.y) * a.heads_per_block + group % a.heads_per_block;
+    const int which = head < q_end ? 0 : head < k_end ? 1 : 2;
+    const Side<T> &side = which == 0 ? a.q : which == 1 ? a.k : a.v;
+    const int n = head - (which == 0 ? 0 : which == 1 ? q_end : k_end);
+    const T *const in = side.in + n * side.is[2];
+    T *const out = side.out + n * side.os[2];
+    const int token_lane = group / a.heads_per_block;
+    const bool active = token_lane < a.token_lanes && n < side.heads;
+    V *const own = staged + threadIdx.x;
+    for (int c0 = 0; c0 < a.chunks; c0 += a.lane_chunks) {
+        const int c = c0 + lane;
+        const bool turns_here = which < 2 && c < a.turned_chunks;
+        Chunk part = {-1, -1};
+        if (turns_here)
+            part = turned_chunk<VEC, INTER>(c, 2 * half);
+        else if (which < 2 && c < a.qk_chunks)
+            part = copied_chunk<VEC>(c - a.turned_chunks, 2 * half, static_cast<int>(a.head_dim));
+        else if (which == 2 && c < a.v_chunks)
+            part = copied_chunk<VEC>(c, 0, static_cast<int>(a.v_dim));
+        const int t0 = active && part.first >= 0 ? token_lane : tile;
+        V *to = own;
+        for (int t = t0; t < tile; t += a.token_lanes) {
+            const T *const from = in + places[t].in[which];
+            copy_in<sizeof(V)>(to, from + part.first);
+            if (part.second >= 0) copy_in<sizeof(V)>(to + blockDim.x, from + part.second);
+            to += 2 * blockDim.x;
+        }
+        if (c0 == 0) {
+            if (threadIdx.x < tile) {
+                row += s;
+                if (!a.positions) position = a.start + row;
+                bool taken = true;
+                if (a.append) {
+                    const bool room = row >= 0 && row < a.capacity;
+                    taken = s < given && room;
+                    if (a.status && blockIdx.y == 0) {
+                        if (given < 0 || given > a.tokens) atomicOr(a.status, LEVO_APPEND_BAD_COUNT);
+                        if (s < given && !room && a.k.heads + a.v.heads > 0) atomicOr(a.status, LEVO_APPEND_NO_ROOM);
+                    }
+                }
+                Place &p = places[threadIdx.x];
+                p.out[0] = b * a.q.os[0] + s * a.q.os[1];
+                p.out[1] = taken ? b * a.k.os[0] + row * a.k.os[1] : -1;
+                p.out[2] = taken ? b * a.v.os[0] + row * a.v.os[1] : -1;
+                p.position = static_cast<double>(position);
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < tile * half; i += blockDim.x) {
+                const int t = i / half, p = i - t * half;
+                const Turn turn = turn_at(places[t].position, i < blockDim.x ? first_theta : a.theta[p], a.magnitude, a.adjoint != 0);
+                float *const at = reinterpret_cast<float *>(turns + t * kPairs2 * a.turned_chunks) +
+                                  turn_slot<VEC, INTER>(p, a.turned_chunks);
+                at[0] = turn.c;
+                at[2] = turn.s;
+            }
+            __syncthreads();
+        }
+        cp_async_wait_all();
+        to = own;
+        for (int t = t0; t < tile; t += a.token_lanes, to += 2 * blockDim.x) {
+            const int64_t at = places[t].out[which];
+            if (at < 0) continue;
+            V x[2] = {to[0], to[blockDim.x]};
+            if (turns_here) turn_pairs<T, VEC, INTER>(x, turns + t * kPairs2 * a.turned_chunks + c, a.turned_chunks);
+            *reinterpret_cast<V *>(out + at + part.first) = x[0];
+            if (part.second >= 0) *reinterpret_cast<V *>(out + at + part.second) = x[1];
+        }
+    }
+}
+
+// Values that every pointer, stride and extent of the call allows in one access (16 bytes at most).
+template <typename T>
+int vector_width(const RopeArgs<T> &a) {
+    int vec = 16 / static_cast<int>(sizeof(T));
+    auto fits = [&](const Side<T> &s, int64_t rows, int64_t dim) {
+        if (s.heads == 0) return true;
+        const int64_t in_size[3] = {a.batch, a.tokens, s.heads}, out_size[3] = {a.batch, rows, s.heads};
+        bool ok = aligned_to(s.in, vec * sizeof(T)) && aligned_to(s.out, vec * sizeof(T)) && dim % vec == 0;
+        for (int i = 0; i < 3; ++i)
+            ok = ok && (in_size[i] <= 1 || s.is[i] % vec == 0) && (out_size[i] <= 1 || s.os[i] % vec == 0);
+        return ok;
+    };
+    const int64_t rows = a.append ? a.capacity : a.tokens;
+    for (; vec > 1; vec /= 2)
+        if ((a.interleaved ? a.rotary_dim : a.rotary_dim / 2) % vec == 0 && fits(a.q, a.tokens, a.head_dim) &&
+            fits(a.k, rows, a.head_dim) && fits(a.v, rows, a.v_dim))
+            break;
+    return vec;
+}
+
+template <typename T, int VEC>
+int launch_width(RopeArgs<T> &a, const char *what, cudaStream_t stream) {
+    constexpr int kPairs2 = (VEC + 1) / 2, kItems = std::min<int>(8, kBytesInFlight / (2 * sizeof(Vec<T, VEC>)));
+    auto half_up = [](int64_t n) { return static_cast<int>((n + 1) / 2); };
+    a.turned_chunks = a.interleaved && VEC > 1 ? half_up(a.rotary_dim / VEC) : static_cast<int>(a.rotary_dim / 2 / VEC);
+    a.qk_chunks = a.turned_chunks + half_up((a.head_dim - a.rotary_dim) / VEC);
+    a.v_chunks = half_up(a.v_dim / VEC);
+    a.chunks = std::max(a.qk_chunks, a.v_chunks);
+    const int64_t tokens = a.batch * a.tokens, heads = a.q.heads + a.k.heads + a.v.heads;
+    if (tokens > INT32_MAX)
+        return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": too many tokens for one call");
+    a.all_tokens = static_cast<uint32_t>(tokens);
+    // Threads of a CTA: chunks x heads x token lanes; each goes through up to kItems tokens.
+    a.lane_chunks = std::min(a.chunks, kMaxThreads);
+    const int64_t enough = 2LL * sm_count();  // CTAs, before heads share one
+    const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(kMaxThreads / a.lane_chunks, tokens * heads / enough));
+    const int64_t groups = (heads + fit - 1) / fit;
+    a.heads_per_block = static_cast<int>((heads + groups - 1) / groups);
+    const int64_t lanes = std::max(1, 256 / (a.lane_chunks * a.heads_per_block));
+    const int per_token = kPairs2 * a.turned_chunks * static_cast<int>(sizeof(Turns2));
+    const int64_t most = std::min<int64_t>({tokens, kMaxTile, std::max<int64_t>(1, kMaxTurns * 8 / per_token)});
+    a.token_lanes = static_cast<int>(std::min(lanes, most));
+    const int64_t items = std::max<int64_t>(1, std::min<int64_t>(kItems, tokens * groups / (a.token_lanes * 4LL * sm_count())));
+    a.tile = static_cast<int>(std::min(most, a.token_lanes * items));
+    const int threads = std::max(32, (a.lane_chunks * a.heads_per_block * a.token_lanes + 31) / 32 * 32);
+    const int64_t blocks = (tokens + a.tile - 1) / a.tile;
+    if (groups > 65535)
+        return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": too many heads for one call");
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(groups));
+    const int passes = (a.tile + a.token_lanes - 1) / a.token_lanes;
+    const size_t smem = static_cast<size_t>(a.tile) * per_token + static_cast<size_t>(passes) * 2 * threads * sizeof(Vec<T, VEC>);
+    auto *const kernel = a.interleaved ? rope_kernel<T, VEC, true> : rope_kernel<T, VEC, false>;
+    int per_sm = 0;
+    if (smem > 48 * 1024 && resident_ctas(reinterpret_cast<const void *>(kernel), threads, smem, &per_sm) != cudaSuccess)
+        return check_launch(what);
+    kernel<<<grid, threads, smem, stream>>>(a);
+    return check_launch(what);
 }
 
 template <typename T>
@@ -182,7 +426,7 @@ int launch_rope(const levo_rope &r, const levo_rope_append *ap, const char *what
     a.tokens = r.tokens;
     a.head_dim = r.head_dim;
     a.rotary_dim = r.rotary_dim;
-    a.v_dim = ap ? ap->v_dim : 0;
+    a.v_dim = ap && ap->v.heads ? ap->v_dim : 0;
     a.theta = r.theta;
     a.positions = r.positions;
     a.ps[0] = r.position_stride[0];
@@ -198,14 +442,16 @@ int launch_rope(const levo_rope &r, const levo_rope_append *ap, const char *what
         a.counts = ap->counts;
         a.status = ap->status;
     }
-    const int64_t units = std::max(r.rotary_dim / 2 + (r.head_dim - r.rotary_dim), a.v_dim);
-    const int64_t total = r.batch * r.tokens * (a.q.heads + a.k.heads + a.v.heads) * units;
-    const int64_t grid = std::min<int64_t>((total + kThreads - 1) / kThreads, int64_t(1) << 30);
-    rope_kernel<T><<<static_cast<unsigned>(grid), kThreads, 0, stream>>>(a);
-    return check_launch(what);
+    switch (vector_width(a)) {
+        case 8: return launch_width<T, 16 / sizeof(T) < 8 ? 4 : 8>(a, what, stream);
+        case 4: return launch_width<T, 4>(a, what, stream);
+        case 2: return launch_width<T, 2>(a, what, stream);
+        default: return launch_width<T, 1>(a, what, stream);
+    }
 }
 
 constexpr int64_t kMaxSize = int64_t(1) << 31;  // of a batch, a token count, a head count or a dimension
+constexpr int64_t kMaxDim = 2 * kMaxTurns;      // a token's sines and cosines fit a CTA's shared memory
 constexpr int64_t kMaxSpan = int64_t(1) << 60;  // of a stride times its size
 constexpr double kMaxWork = 1e16;               // values of one call: its counters stay inside 64 bits
 
@@ -274,6 +520,8 @@ int check_rope(const char *what, const levo_rope &r, size_t *element) {
 }
 
 int dispatch(const levo_rope &r, const levo_rope_append *ap, const char *what, levo_stream_t stream) {
+    if (r.head_dim > kMaxDim || (ap && ap->v.heads && ap->v_dim > kMaxDim))
+        return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": head dimension above 8192");
     const double width = static_cast<double>(std::max(r.head_dim, ap ? ap->v_dim : 0));
     const double heads = static_cast<double>(r.q.heads + r.k.heads + (ap ? ap->v.heads : 0));
     if (static_cast<double>(r.batch) * static_cast<double>(r.tokens) * heads * width > kMaxWork)
