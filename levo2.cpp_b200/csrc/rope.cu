@@ -399,8 +399,10 @@ int launch_width(RopeArgs<T> &a, const char *what, cudaStream_t stream) {
         return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": too many heads for one call");
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(groups));
     const int passes = (a.tile + a.token_lanes - 1) / a.token_lanes;
-    const size_t smem = static_cast<size_t>(a.tile) * per_token + static_cast<size_t>(passes) * 2 * threads * sizeof(Vec<T, VEC>);
+    // Above 48 KB with the static part the kernel has to opt in, which resident_ctas does from the dynamic part alone.
+    size_t smem = static_cast<size_t>(a.tile) * per_token + static_cast<size_t>(passes) * 2 * threads * sizeof(Vec<T, VEC>);
     auto *const kernel = a.interleaved ? rope_kernel<T, VEC, true> : rope_kernel<T, VEC, false>;
+    if (smem + kMaxTile * sizeof(Place) > 48 * 1024) smem = std::max<size_t>(smem, 48 * 1024 + 16);
     int per_sm = 0;
     if (smem > 48 * 1024 && resident_ctas(reinterpret_cast<const void *>(kernel), threads, smem, &per_sm) != cudaSuccess)
         return check_launch(what);
