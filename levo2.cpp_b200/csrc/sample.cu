@@ -84,10 +84,9 @@ constexpr double ln2_coefficient(int k) {
     return c;
 }
 
-__device__ __forceinline__ u64 weight_of(float v, float top, double scale) {
-    if (v == top) return 1ull << 44;
-    const double x = (static_cast<double>(v) - static_cast<double>(top)) * scale;
-    if (!(x > -46.0)) return 0;
+// For v within 32 T of the top, as bin_of takes them: x > -47.
+__device__ __forceinline__ u64 weight_of(float v, double top, double scale) {
+    const double x = (static_cast<double>(v) - top) * scale;
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
     const double r = x + kRound;
     const double f = x - (r - kRound);
@@ -110,7 +109,7 @@ struct Shared {
     u64 passing[kMaxCluster];         // first CTA: weight that min-p leaves, of each CTA
     Found found;
     u64 target;
-    u64 before;                       // of the slice that the target falls into
+    u64 before, upto;                 // the slice that the target falls into: what lies before it, and with it
     int bin;
     int cursor[kSearches];            // first CTA: tokens of each list
     uint32_t most[kMaxCluster], least[kMaxCluster], ties[kMaxCluster];  // of every CTA, in every CTA
@@ -159,11 +158,10 @@ class Row {
         load();
         share_extremes();
         settings();
-        if (top == -INFINITY) {
-            if (leader()) finish(-1, 0, 1);
-        } else {
+        if (top == -INFINITY)
+            finish(-1, 0, 1);
+        else
             sample();
-        }
         sync_all();  // nobody leaves while another reads its shared memory
     }
 
@@ -178,8 +176,8 @@ class Row {
     int64_t row;
     int start, count, phase, quads;  // first logit and number of this CTA's, offset of the first in buf, float4s of buf
     float top, lowest;               // largest and smallest logit above -inf
-    float half_top, reach, slices;   // (top - v) / 2 up to `reach` has weight; slices of it a unit
-    double scale;
+    float half_top, slices;          // slices of a unit of (top - v) / 2
+    double wide_top, scale;
     int64_t top_k;
     float top_p, min_p, uniform;
     bool bad;
@@ -334,39 +332,56 @@ class Row {
         if (!(uniform >= 0.0f && uniform < 1.0f)) bad = true, uniform = uniform >= 1.0f ? 1.0f : 0.0f;
         if (temperature == 0.0f) top_k = 1;
         scale = temperature > 0.0f ? 1.4426950408889634074 / static_cast<double>(temperature) : 0.0;
-        // Half differences, so that none overflows.  31.9 T and more below the maximum there is no weight (2^-46).
+        if (top == INFINITY) {  // +inf alone has weight: as 0 among -inf
+            for (int g = tid; g < quads; g += kThreads) {
+                float4 &q = reinterpret_cast<float4 *>(buf)[g];
+                q.x = q.x == top ? 0.0f : -INFINITY, q.y = q.y == top ? 0.0f : -INFINITY;
+                q.z = q.z == top ? 0.0f : -INFINITY, q.w = q.w == top ? 0.0f : -INFINITY;
+            }
+            top = lowest = 0.0f;
+            __syncthreads();
+        }
+        // Half differences, so that none overflows.  The slices reach to the lowest logit, or to 31.9 T below the top,
+        // where weights are below 2^-45 and round to nothing.
         half_top = 0.5f * top;
-        reach = isinf(top) ? 0.0f : fminf(__fmaf_rn(-0.5f, lowest, half_top), 15.95f * temperature);
-        slices = fminf(__fdiv_rn(static_cast<float>(kBins), reach), FLT_MAX);
+        wide_top = top;
+        const float reach = fminf(__fmaf_rn(-0.5f, lowest, half_top), 15.95f * temperature);
+        slices = fminf(__fdiv_rn(static_cast<float>(kBins - 1), reach), FLT_MAX);
     }
 
-    // Slice of a logit (never larger for a larger logit), or -1 where it has no weight.
-    __device__ int bin_of(float v) const {
-        const float d = v == top ? 0.0f : __fmaf_rn(-0.5f, v, half_top);
-        if (!(d <= reach)) return -1;
-        return min(kBins - 1, static_cast<int>(d * slices));
+    // Slice of a logit: never smaller for a smaller logit; kBins and above where there is no weight (-inf among it).
+    // The sum with 2^23 leaves the nearest integer in the low bits.
+    __device__ uint32_t bin_of(float v) const {
+        const float d = __fmaf_rn(-0.5f, v, half_top);
+        return __float_as_uint(__fmaf_rn(d, slices, 8388608.0f)) - 0x4b000000u;
     }
     __device__ bool within(float v, int index) const {
-        return !limited || v > limit_value || (v == limit_value && index <= limit_index);
+        return v > limit_value || (v == limit_value && index <= limit_index);
     }
-    __device__ u64 weight(float v) const { return weight_of(v, top, scale); }
+    __device__ u64 weight(float v) const { return weight_of(v, wide_top, scale); }
 
-    // f(logit, index, slice) for every token of this CTA that has weight and that top-k has left.
+    // f(logits, slices, index of the first) for this CTA's tokens by fours; a token without weight, or beyond the
+    // limit of top-k, has a slice of kBins or above.
     template <typename F>
-    __device__ void for_each(F f) {
+    __device__ void for_fours(F f) {
         for (int g = tid; g < quads; g += kThreads) {
             const float4 q = reinterpret_cast<const float4 *>(buf)[g];
             const float v[4] = {q.x, q.y, q.z, q.w};
+            const int first = start + 4 * g - phase;
+            uint32_t bin[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int bin = bin_of(v[i]), index = start + 4 * g + i - phase;
-                if (bin >= 0 && within(v[i], index)) f(v[i], index, bin);
+            for (int i = 0; i < 4; ++i) bin[i] = bin_of(v[i]);
+            if (limited) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!within(v[i], first + i)) bin[i] = kBins;
             }
+            f(v, bin, first);
         }
     }
 
     // ---- histograms ----------------------------------------------------------------------------------------
-    __device__ void add(int bin, u64 w) {
+    __device__ void add(uint32_t bin, u64 w) {
         const uint32_t low = static_cast<uint32_t>(w);
         const uint32_t old = atomicAdd(&lo[bin], low);
         const uint32_t high = static_cast<uint32_t>(w >> 32) + (old + low < old);
@@ -396,19 +411,8 @@ class Row {
             own[i] = CLUSTER ? scan[bin] : (static_cast<u64>(hi[bin]) << 32) + lo[bin];
             sum += own[i];
         }
-        u64 upto = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const u64 v = __shfl_up_sync(0xffffffffu, upto, o);
-            if ((tid & 31) >= o) upto += v;
-        }
-        if ((tid & 31) == 31) sh.warp_sums[tid >> 5] = upto;
-        __syncthreads();
-        u64 before = upto - sum, all = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w == (tid >> 5)) before += all;
-            all += sh.warp_sums[w];
-        }
+        u64 all;
+        u64 before = sum_before(sum, all);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             scan[tid * kEach + i] = before;
@@ -431,6 +435,7 @@ class Row {
                         Shared &to = *at(&sh, c);
                         to.bin = bin;
                         to.before = scan[bin];
+                        to.upto = next;
                         to.target = target;
                     }
             }
@@ -438,68 +443,117 @@ class Row {
         sync_all();
     }
 
-    // Collects the tokens that `member` takes in the first CTA's list; returns how many there are (kList are held).
-    template <typename M>
-    __device__ int collect(M member) {
+    // Collects the tokens whose slice lies in [from, to] and whose key in [low, high] in the first CTA's list; returns
+    // how many there are (kList are held).
+    __device__ int collect(uint32_t from, uint32_t to, uint32_t low = 0, uint32_t high = 0xffffffffu) {
         int *const cursor = at(&sh.cursor[searches], 0);
-        u64 *const to = at(list, 0);
-        for_each([&](float v, int index, int bin) {
-            if (!member(v, bin)) return;
-            const int place = atomicAdd(cursor, 1);
-            if (place < kList) to[place] = order_of(v, index);
+        u64 *const into = at(list, 0);
+        for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int first) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= bin[i] - from <= to - from;
+            if (!any) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t key = key_of(v[i]);
+                if (bin[i] - from > to - from || key < low || key > high) continue;
+                const int place = atomicAdd(cursor, 1);
+                if (place < kList) into[place] = order_of(v[i], first + i);
+            }
         });
         sync_all();
         ++searches;
         return *cursor;
     }
 
-    // First CTA: which of the n listed tokens the target falls into.  Several threads a token add up the list.
-    __device__ void rank_list(int n, u64 before, u64 target, bool by_weight) {
-        for (int i = tid; i < n; i += kThreads)
-            list_own[i] = by_weight ? weight(value_of(~static_cast<uint32_t>(list[i] >> 32))) : 1;
+    // First CTA: the n listed tokens in order, one a thread (all ones behind them).  A bitonic network: strides below a
+    // warp by shuffles, the others through two arrays in turn.
+    __device__ u64 sorted(int n) {
+        u64 mine = tid < n ? list[tid] : ~0ull;
+        u64 *area = list_own, *next = list;
         __syncthreads();
-        int share = 32;
-        while (share > 1 && n * share > kThreads) share >>= 1;
-        const int lane = tid % share;
-        for (int i = tid / share; i - tid / share < n; i += kThreads / share) {
-            const u64 mine = i < n ? list[i] : 0;
-            u64 sum = 0;
-            for (int j = lane; j < n; j += share)
-                if (list[j] < mine) sum += list_own[j];
-            for (int o = share / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0 && i < n && before + sum <= target && target < before + sum + list_own[i])
-                sh.found = {mine, before + sum, list_own[i]};
+        for (int size = 2; size < 2 * n; size <<= 1)
+            for (int stride = size >> 1; stride > 0; stride >>= 1) {
+                u64 other;
+                if (stride >= 32) {
+                    area[tid] = mine;
+                    __syncthreads();
+                    other = area[tid ^ stride];
+                    u64 *const t = area;
+                    area = next;
+                    next = t;
+                } else {
+                    other = __shfl_xor_sync(0xffffffffu, mine, stride);
+                }
+                const bool smaller = ((tid & stride) == 0) == ((tid & size) == 0);
+                if ((other < mine) == smaller) mine = other;
+            }
+        __syncthreads();
+        return mine;
+    }
+
+    // Running sum over the CTA's threads (what lies before this one); `all`: the whole.
+    __device__ u64 sum_before(u64 own, u64 &all) {
+        u64 upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 v = __shfl_up_sync(0xffffffffu, upto, o);
+            if ((tid & 31) >= o) upto += v;
         }
+        if ((tid & 31) == 31) sh.warp_sums[tid >> 5] = upto;
+        __syncthreads();
+        u64 before = upto - own;
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == (tid >> 5)) before += all;
+            all += sh.warp_sums[w];
+        }
+        __syncthreads();
+        return before;
+    }
+
+    static __device__ float value_in(u64 order) { return value_of(~static_cast<uint32_t>(order >> 32)); }
+    static __device__ int index_in(u64 order) { return static_cast<int>(static_cast<uint32_t>(order)); }
+
+    // First CTA: which of the n listed tokens the target falls into.
+    __device__ void rank_list(int n, u64 before, u64 target, bool by_weight) {
+        const u64 mine = sorted(n);
+        const u64 own = tid >= n ? 0 : by_weight ? weight(value_in(mine)) : 1;
+        u64 all;
+        const u64 sum = before + sum_before(own, all);
+        if (sum <= target && target < sum + own) sh.found = {mine, sum, own};
         __syncthreads();
     }
 
-    // The token that `target` falls into: in the first CTA's sh.found.  running_sums() went before; a slice with too
-    // many tokens costs the histogram (returns false then).
-    __device__ bool search(u64 target, bool by_weight) {
-        locate(target);
-        const int bin = sh.bin;
+    // The token of the located slice that the target falls into: in the first CTA's sh.found.  A slice with too many
+    // tokens costs the histogram (returns false then).
+    __device__ bool search_slice(bool by_weight) {
+        const uint32_t slice = sh.bin;
         u64 before = sh.before;
-        target = sh.target;
-        int n = collect([&](float, int b) { return b == bin; });
+        const u64 target = sh.target;
+        int n = collect(slice, slice);
         if (n <= kList) {
             if (leader()) rank_list(n, before, target, by_weight);
             return true;
         }
         uint32_t low_key = 0, high_key = 0xffffffffu;
         for (;;) {
-            auto member = [&](float v, int b) {
+            auto member = [&](float v, uint32_t bin) {
                 const uint32_t key = key_of(v);
-                return b == bin && key >= low_key && key <= high_key;
+                return bin == slice && key >= low_key && key <= high_key;
             };
             // keys of the slice that is left
             uint32_t most = 0, least = 0xffffffffu, group = 0;
             if (tid == 0) sh.block_most = 0, sh.block_least = 0xffffffffu;
             clear_bins();
             __syncthreads();
-            for_each([&](float v, int, int b) {
-                if (!member(v, b)) return;
-                most = max(most, key_of(v)), least = min(least, key_of(v));
-                ++group;
+            for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int) {
+                for (int i = 0; i < 4; ++i)
+                    if (member(v[i], bin[i])) {
+                        most = max(most, key_of(v[i])), least = min(least, key_of(v[i]));
+                        ++group;
+                    }
             });
             most = __reduce_max_sync(0xffffffffu, most);
             least = __reduce_min_sync(0xffffffffu, least);
@@ -535,15 +589,16 @@ class Row {
             }
             int shift = 0;
             while (((most - least) >> shift) >= kBins) ++shift;
-            for_each([&](float v, int, int b) {
-                if (member(v, b)) add(static_cast<int>((most - key_of(v)) >> shift), by_weight ? weight(v) : 1);
+            for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int) {
+                for (int i = 0; i < 4; ++i)
+                    if (member(v[i], bin[i])) add((most - key_of(v[i])) >> shift, by_weight ? weight(v[i]) : 1);
             });
             running_sums();
             locate(target - before);
             before += sh.before;
             high_key = most - (static_cast<uint32_t>(sh.bin) << shift);
             low_key = max(least, high_key - ((1u << shift) - 1));
-            n = collect(member);
+            n = collect(slice, slice, low_key, high_key);
             if (n <= kList) {
                 if (leader()) rank_list(n, before, target, by_weight);
                 return false;
@@ -573,60 +628,105 @@ class Row {
     }
 
     // ---- the filters and the draw ----------------------------------------------------------------------------
+    __device__ u64 least_weight() const {
+        return static_cast<u64>(ceil(static_cast<double>(min_p) * 17592186044416.0));  // 2^44
+    }
+
+    // The histogram of weights and its running sums; what min-p leaves of them to the first CTA.
     __device__ void weigh() {
-        const u64 least = static_cast<u64>(ceil(static_cast<double>(min_p) * 17592186044416.0));  // 2^44
+        const u64 least = least_weight();
         u64 passing = 0;
-        for_each([&](float v, int, int bin) {
-            const u64 w = weight(v);
-            add(bin, w);
-            if (w >= least) passing += w;
+        for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int) {
+            if (bin[0] >= kBins && bin[1] >= kBins && bin[2] >= kBins && bin[3] >= kBins) return;
+            u64 w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = weight(bin[i] < kBins ? v[i] : top);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (bin[i] < kBins) {
+                    add(bin[i], w[i]);
+                    if (w[i] >= least) passing += w[i];
+                }
         });
         if (min_p > 0.0f) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) passing += __shfl_xor_sync(0xffffffffu, passing, o);
-            __syncthreads();
-            if ((tid & 31) == 0) sh.warp_sums[tid >> 5] = passing;
-            __syncthreads();
-            if (tid == 0) {
-                u64 all = 0;
-                for (int w = 0; w < kWarps; ++w) all += sh.warp_sums[w];
-                at(&sh, 0)->passing[rank] = all;
-            }
+            u64 all;
+            sum_before(passing, all);
+            if (tid == 0) at(&sh, 0)->passing[rank] = all;
         }
         running_sums();
     }
 
+    // Weight that is kept of `all`: up to the token that passes top-p, and no more than min-p lets pass.
+    __device__ u64 drawn(u64 kept) const {
+        const u64 place = static_cast<u64>(static_cast<double>(uniform) * static_cast<double>(kept));
+        return min(place, kept - 1);
+    }
+    __device__ u64 nucleus(u64 all) const {  // the weight whose token is the last that top-p keeps
+        const u64 part = static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(all)));
+        return max(part, u64(1)) - 1;
+    }
+
+    // First CTA: all that can be drawn is in the list (n tokens and no more): filters and draw over it in order.
+    __device__ void sample_list(int n) {
+        const u64 mine = sorted(n);
+        const u64 own = tid < min(static_cast<int64_t>(n), top_k) ? weight(value_in(mine)) : 0;
+        u64 kept, passing;
+        const u64 before = sum_before(own, kept);
+        if (top_p < 1.0f) {
+            const u64 target = nucleus(kept);
+            if (before <= target && target < before + own) sh.total = before + own;
+            __syncthreads();
+            kept = sh.total;
+        }
+        if (min_p > 0.0f) {
+            sum_before(own >= least_weight() ? own : 0, passing);
+            kept = min(kept, passing);
+        }
+        const u64 target = drawn(kept);
+        if (before <= target && target < before + own) sh.found = {mine, before, own};
+        __syncthreads();
+        finish(index_in(sh.found.order), sh.found.own, kept);
+    }
+
     __device__ void sample() {
+        if (a.vocab <= kList) {
+            const int n = collect(0, kBins - 1);
+            if (leader()) sample_list(n);
+            return;
+        }
         if (top_k < a.vocab) {
-            for_each([&](float, int, int bin) { atomicAdd(&lo[bin], 1u); });
+            for_fours([&](const float(&)[4], const uint32_t(&bin)[4], int) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (bin[i] < kBins) atomicAdd(&lo[bin[i]], 1u);
+            });
             running_sums();
-            sync_all();  // every CTA asks for the total of the first
-            const bool cuts = *at(&sh.total, 0) > static_cast<u64>(top_k);
-            if (cuts) {
-                search(static_cast<u64>(top_k) - 1, false);
+            locate(leader() ? min(static_cast<u64>(top_k), sh.total) - 1 : 0);
+            // The k-th token's slice, or the last one with a token.  Few enough up to it: the first CTA has them all.
+            if (sh.upto <= kList) {
+                const int n = collect(0, sh.bin);
+                if (leader()) sample_list(n);
+                return;
+            }
+            if (sh.target + 1 == static_cast<u64>(top_k)) {
+                search_slice(false);
                 if (CLUSTER) {
                     if (leader() && tid > 0 && tid < ctas) at(&sh, tid)->found = sh.found;
                     sync_all();
                 }
                 limited = true;
-                limit_value = value_of(~static_cast<uint32_t>(sh.found.order >> 32));
-                limit_index = static_cast<int>(static_cast<uint32_t>(sh.found.order));
-                if (top_k == 1) {
-                    if (leader()) finish(limit_index, 1, 1);
-                    return;
-                }
+                limit_value = value_in(sh.found.order);
+                limit_index = index_in(sh.found.order);
             }
-            __syncthreads();
-            if (CLUSTER) sync_all();  // the histograms have been read
+            sync_all();  // the histograms have been read
             clear_bins();
             __syncthreads();
         }
         weigh();
         u64 kept = leader() ? sh.total : 0;
         if (top_p < 1.0f) {
-            const double part = ceil(static_cast<double>(top_p) * static_cast<double>(kept));
-            const u64 target = leader() ? max(1ull, static_cast<u64>(part)) - 1 : 0;
-            const bool whole = search(target, true);
+            locate(leader() ? nucleus(kept) : 0);
+            const bool whole = search_slice(true);
             kept = leader() ? sh.found.before + sh.found.own : 0;
             if (!whole) {
                 sync_all();
@@ -640,14 +740,13 @@ class Row {
             for (int c = 0; c < ctas; ++c) passing += sh.passing[c];
             kept = min(kept, passing);
         }
-        const u64 target =
-            leader() ? min(static_cast<u64>(static_cast<double>(uniform) * static_cast<double>(kept)), kept - 1) : 0;
-        search(target, true);
-        if (leader()) finish(static_cast<int>(static_cast<uint32_t>(sh.found.order)), sh.found.own, kept);
+        locate(leader() ? drawn(kept) : 0);
+        search_slice(true);
+        finish(index_in(sh.found.order), sh.found.own, kept);
     }
 
     __device__ void finish(int token, u64 own, u64 kept) {
-        if (tid != 0) return;
+        if (!leader() || tid != 0) return;
         a.out[row] = max(token, 0);
         if (a.logprob)
             a.logprob[row] = token < 0 ? -INFINITY
