@@ -38,9 +38,12 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBins = 2048;
+constexpr int kBins = 4096;      // slices of a histogram of weights
+constexpr int kCountBins = 512;  // and of one of counts
 constexpr int kList = 512;
+static_assert(kList == kThreads, "a listed token a thread");
 constexpr int kMaxCluster = 8;
+constexpr int kRing = 8;  // groups that a thread has on their way when it reads a row again
 constexpr int kSearches = 16;  // lists of one row: three searches, each with up to three further cuts
 constexpr int64_t kMaxVocab = int64_t(1) << 17;
 
@@ -58,12 +61,12 @@ struct SampleArgs {
     int64_t *out;
     float *logprob;
     int32_t *status;
-    int chunk, slots;  // logits of a CTA, and its places in shared memory
+    int chunk, slots, words;  // logits of a CTA, their places and the words of their bits in shared memory
 };
 
-// Integers in the order of the values (-0 and +0 are made one before).
+// Integers in the order of the values (-0 is made +0).
 __device__ __forceinline__ uint32_t key_of(float v) {
-    const uint32_t b = __float_as_uint(v);
+    const uint32_t b = __float_as_uint(v + 0.0f);
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 __device__ __forceinline__ float value_of(uint32_t key) {
@@ -74,28 +77,47 @@ __device__ __forceinline__ u64 order_of(float v, int index) {
     return (static_cast<u64>(~key_of(v)) << 32) | static_cast<uint32_t>(index);
 }
 
-// exp((v - top) / T) in units of 2^-44: 2^x, x = (v - top) * log2(e)/T in F64, as
-// 2^n (n the nearest integer) times the Taylor series of 2^f, |f| <= 1/2, to
-// degree 10 (the first term left out is (ln2/2)^11 / 11! = 2.2e-13).
+// exp((v - top) / T) in units of 2^-44.  y = (v - top) * 64 log2(e)/T in F64, k the
+// nearest integer, g = y - k: 2^(44 + k/64), from a table of 2^(44 + j/64), times the
+// Taylor series of 2^(g/64), |g| <= 1/2, to degree 4 (the first term left out is
+// (ln2/128)^5 / 5! = 3.9e-14, below the unit).
+constexpr int kSteps = 64;
 constexpr double kLn2 = 0.693147180559945309417;
-constexpr double ln2_coefficient(int k) {
+constexpr double step_coefficient(int k) {  // of g^k
     double c = 1.0;
-    for (int i = 1; i <= k; ++i) c *= kLn2 / i;
+    for (int i = 1; i <= k; ++i) c *= kLn2 / kSteps / i;
     return c;
 }
 
-// For v within 32 T of the top, as bin_of takes them: x > -47.
-__device__ __forceinline__ u64 weight_of(float v, double top, double scale) {
-    const double x = (static_cast<double>(v) - top) * scale;
+// 2^(44 + j/64): the Taylor series of 2^f, |f| <= 1/2, to degree 18, as the compiler evaluates it.
+struct StepPowers {
+    double v[kSteps];
+    constexpr StepPowers() : v() {
+        for (int j = 0; j < kSteps; ++j) {
+            const double x = kLn2 * (j < kSteps / 2 ? j : j - kSteps) / kSteps;
+            double p = 1.0;
+            for (int k = 18; k > 0; --k) p = 1.0 + p * x / k;
+            v[j] = p * (j < kSteps / 2 ? 17592186044416.0 : 35184372088832.0);
+        }
+    }
+};
+__device__ const StepPowers kStepPowers{};
+
+// For v within 32 T of the top, as bin_of takes them: the result is below 2^45 and its exponent above -3.
+__device__ __forceinline__ u64 weight_of(float v, double top, double scale, const double *powers) {
+    const double y = (static_cast<double>(v) - top) * scale;
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
-    const double r = x + kRound;
-    const double f = x - (r - kRound);
-    double p = ln2_coefficient(10);
-#pragma unroll
-    for (int k = 9; k >= 0; --k) p = __fma_rn(p, f, ln2_coefficient(k));
-    // p * 2^(44 + n) <= 2^44: adding 2^52 rounds it to an integer in the low mantissa bits
-    const double scaled = __hiloint2double(__double2hiint(p) + ((__double2loint(r) + 44) << 20), __double2loint(p));
-    return static_cast<u64>(__double_as_longlong(scaled + 4503599627370496.0)) & ((1ull << 52) - 1);
+    const double r = y + kRound;
+    const int k = __double2loint(r);
+    const double g = y - (r - kRound);
+    double p = __fma_rn(step_coefficient(4), g, step_coefficient(3));
+    p = __fma_rn(p, g, step_coefficient(2));
+    p = __fma_rn(p, g, step_coefficient(1)) * g;
+    const double power = powers[k & (kSteps - 1)];
+    const double t = __hiloint2double(__double2hiint(power) + ((k & -kSteps) << 14), __double2loint(power));
+    // adding 2^52 rounds to an integer in the low mantissa bits
+    const double w = __fma_rn(t, p, t) + 4503599627370496.0;
+    return static_cast<u64>(__double_as_longlong(w)) & ((1ull << 52) - 1);
 }
 
 // A token found: its place in the order, what lies before it, and what it has itself (weight, or 1).
@@ -104,11 +126,13 @@ struct Found {
 };
 
 struct Shared {
+    double powers[kSteps];
     u64 warp_sums[kWarps];
     u64 total;                        // first CTA: of the histogram
     u64 passing[kMaxCluster];         // first CTA: weight that min-p leaves, of each CTA
     Found found;
     u64 target;
+    int place;                        // of this CTA's first token in the list
     u64 before, upto;                 // the slice that the target falls into: what lies before it, and with it
     int bin;
     int cursor[kSearches];            // first CTA: tokens of each list
@@ -117,6 +141,7 @@ struct Shared {
     uint32_t block_most, block_least;
     int block_nan;
     int warp_counts[kWarps];
+    int places[kThreads], ends[kThreads];  // of a list's slices
 };
 
 template <typename T>
@@ -134,17 +159,18 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) {
     return __bfloat162float(v);
 }
 
-template <typename T, bool CLUSTER>
+template <typename T, bool CLUSTER, bool HELD>
 class Row {
    public:
     __device__ Row(const SampleArgs &args, Shared &shared, unsigned char *dynamic) : a(args), sh(shared) {
-        buf = reinterpret_cast<float *>(dynamic);
-        lo = reinterpret_cast<uint32_t *>(buf + a.slots);
+        lo = reinterpret_cast<uint32_t *>(dynamic);
         hi = lo + kBins;
-        scan = reinterpret_cast<u64 *>(hi + kBins);
-        list = scan + kBins;
-        list_own = list + kList;
-        bitmap = reinterpret_cast<uint32_t *>(list_own + kList);
+        list = reinterpret_cast<u64 *>(hi + kBins);
+        spare = list + kList;
+        buf = reinterpret_cast<float *>(spare + kList);
+        ring = reinterpret_cast<uint4 *>(buf);
+        penalised = (HELD ? lo : reinterpret_cast<uint32_t *>(buf + a.slots)) + 1;
+        ignored = penalised + a.words;
         tid = threadIdx.x;
         rank = CLUSTER ? static_cast<int>(cg::this_cluster().block_rank()) : 0;
         ctas = CLUSTER ? static_cast<int>(cg::this_cluster().num_blocks()) : 1;
@@ -153,8 +179,9 @@ class Row {
     __device__ void run(int64_t row_index) {
         row = row_index;
         if (tid < kSearches) sh.cursor[tid] = 0;
+        if (tid < kSteps) sh.powers[tid] = kStepPowers.v[tid];
         if (tid == 0) sh.block_most = 0, sh.block_least = 0xffffffffu, sh.block_nan = 0;
-        clear_bins();
+        ask();
         load();
         share_extremes();
         settings();
@@ -168,19 +195,25 @@ class Row {
    private:
     const SampleArgs &a;
     Shared &sh;
-    float *buf;
-    uint32_t *lo, *hi;  // histogram: 64-bit sums in two words
-    u64 *scan, *list, *list_own;
-    uint32_t *bitmap;
+    uint32_t *lo, *hi;  // histogram, then its running sums (first CTA): 64 bits in two words
+    u64 *list, *spare;
+    float *buf;                     // HELD: this CTA's logits, as the order sees them
+    uint4 *ring;                    // else: groups on their way
+    uint32_t *penalised, *ignored;  // a bit a logit, and a word to spare at both ends (HELD: in the histogram's place)
     int tid, rank, ctas, searches = 0;
     int64_t row;
-    int start, count, phase, quads;  // first logit and number of this CTA's, offset of the first in buf, float4s of buf
-    float top, lowest;               // largest and smallest logit above -inf
-    float half_top, slices;          // slices of a unit of (top - v) / 2
+    const T *x;                       // this CTA's logits
+    int start, count, phase, groups;  // its first, how many, offset of the first from a 16-byte boundary, 16-byte groups
+    bool edits;                       // the row has penalised or ignored ids
+    float top, lowest;                // largest and smallest logit above -inf
+    float thread_top;                 // largest of this thread's
+    float half_top, reach, slices;   // slices of a unit of (top - v) / 2, which has weight up to `reach`
+    int bins;
     double wide_top, scale;
     int64_t top_k;
     float top_p, min_p, uniform;
-    bool bad;
+    float temperature;
+    bool bad, infinite;
     bool limited = false;  // by top-k: tokens up to (limit_value, limit_index) in the order
     float limit_value;
     int limit_index;
@@ -197,96 +230,176 @@ class Row {
         return CLUSTER ? cg::this_cluster().map_shared_rank(mine, cta) : mine;
     }
 
-    __device__ void clear_bins() {
-        uint4 *words = reinterpret_cast<uint4 *>(lo);
-        for (int i = tid; i < 2 * kBins / 4; i += kThreads) words[i] = make_uint4(0, 0, 0, 0);
+    // An empty histogram of that many slices.
+    __device__ void new_bins(int n) {
+        bins = n;
+        slices = fminf(__fdiv_rn(static_cast<float>(n - 1), reach), FLT_MAX);
+        clear();
+    }
+    __device__ void clear() {
+        for (int i = 4 * tid; i < bins; i += 4 * kThreads) {
+            *reinterpret_cast<uint4 *>(lo + i) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(hi + i) = make_uint4(0, 0, 0, 0);
+        }
+        __syncthreads();
     }
 
     // ---- the row -------------------------------------------------------------------------------------------
-    // NaN as -inf (flagged), -0 as +0.
-    __device__ float clean(float v, int &nan) {
-        if (isnan(v)) {
-            nan = 1;
-            return -INFINITY;
+    static constexpr int L = 16 / sizeof(T);  // logits of a 16-byte group
+    // Groups whose loads a thread has on their way.  The whole of a 16384-token vocabulary and of the few tokens that
+    // commonly come on top of a power of two.
+    static constexpr int kAhead = sizeof(T) == 4 ? 9 : 5;
+
+    __device__ bool ignores() const { return a.ignore && (a.streams > 0 ? row % a.streams == 0 : row == 0); }
+
+    // The L bits of a group.
+    __device__ uint32_t bits_of(const uint32_t *words, int g) const {
+        const int e = g * L - phase;
+        return __funnelshift_r(words[e >> 5], words[(e >> 5) + 1], e & 31) & ((1u << L) - 1);
+    }
+    static __device__ __noinline__ float penalty_of(float v, float penalty) { return __fdiv_rn(v, penalty); }
+
+    // A bit for every penalised and every ignored id of this CTA's share.
+    __device__ void mark_edits() {
+        for (int i = tid - 1; i < 2 * a.words - 1; i += kThreads) penalised[i] = 0;
+        __syncthreads();
+        if (a.recent)
+            for (int64_t j = tid; j < a.recent_len; j += kThreads) {
+                const int64_t id = a.recent[row * a.recent_len + j], e = id - start;
+                if (id >= 0 && id < a.limit && e >= 0 && e < count) atomicOr(&penalised[e >> 5], 1u << (e & 31));
+            }
+        if (ignores())
+            for (int64_t j = tid; j < a.n_ignore; j += kThreads) {
+                const int64_t e = a.ignore[j] - start;
+                if (e >= 0 && e < count) atomicOr(&ignored[e >> 5], 1u << (e & 31));
+            }
+        __syncthreads();
+    }
+
+    // f(group, logits, first, end) for each of this CTA's groups, whose logits [first, end) are the CTA's (the others
+    // are -inf); `between` runs while the first loads are on their way.  The same threads take the same groups always.
+    template <typename B, typename F>
+    __device__ void read_groups(B between, F f) {
+        const int begin = phase > 0 ? 1 : 0, end = (phase + count) / L;  // whole groups
+        const T *const base = x - phase;
+        auto take = [&](const uint4 &raw, int g) {
+            const T *values = reinterpret_cast<const T *>(&raw);
+            float v[L];
+#pragma unroll
+            for (int i = 0; i < L; ++i) v[i] = to_float(values[i]);
+            f(g, v);
+        };
+        if constexpr (HELD) {
+            for (int g0 = begin + tid; g0 - tid < end || g0 == begin + tid; g0 += kAhead * kThreads) {
+                uint4 raw[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    if (g0 + j * kThreads < end)
+                        raw[j] = *reinterpret_cast<const uint4 *>(base + (g0 + j * kThreads) * L);
+                if (g0 == begin + tid) between();
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    if (g0 + j * kThreads >= end) break;
+                    take(raw[j], g0 + j * kThreads);
+                }
+            }
+        } else {
+            // a ring of kRing groups a thread in shared memory, which that thread alone fills and reads
+            uint4 *const own = ring + tid;
+            auto start_copy = [&](int g, int slot) {
+                if (g < end) cp_async16(own + slot * kThreads, base + g * L);
+                cp_async_commit();
+            };
+#pragma unroll
+            for (int j = 0; j < kRing; ++j) start_copy(begin + tid + j * kThreads, j);
+            between();
+            int slot = 0;
+            for (int g = begin + tid; g < end; g += kThreads) {
+                cp_async_wait_group<kRing - 1>();
+                const uint4 raw = own[slot * kThreads];
+                start_copy(g + kRing * kThreads, slot);
+                slot = (slot + 1) % kRing;
+                take(raw, g);
+            }
+            cp_async_wait_all();
         }
-        return v + 0.0f;
+        // the parts of a group at both ends
+        const int g = tid == 0 ? 0 : groups - 1;
+        if ((tid == 0 && begin > 0) || (tid == kThreads - 1 && end < groups && (groups > 1 || begin == 0))) {
+            float v[L];
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int e = g * L - phase + i;
+                v[i] = e >= 0 && e < count ? to_float(x[e]) : -INFINITY;
+            }
+            f(g, v);
+        }
+    }
+
+    // Penalty and ignore list of a group read again.
+    __device__ void edit(float (&v)[L], int g) const {
+        const uint32_t p = bits_of(penalised, g), n = bits_of(ignored, g);
+        if (p | n) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                if (p >> i & 1) v[i] = penalty_of(v[i], a.penalty);
+                if (n >> i & 1) v[i] = -INFINITY;
+            }
+        }
     }
 
     __device__ void load() {
-        constexpr int L = 16 / sizeof(T);
         start = rank * a.chunk;
         count = static_cast<int>(min(static_cast<int64_t>(a.chunk), a.vocab - start));
-        const T *x = static_cast<const T *>(a.logits) + row * a.ld + start;
+        x = static_cast<const T *>(a.logits) + row * a.ld + start;
         phase = static_cast<int>(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (L - 1);
-        const int groups = (phase + count + L - 1) / L;  // of 16 bytes; the first and last may be parts
-        quads = groups * L / 4;
-        const bool ignores = a.ignore && (a.streams > 0 ? row % a.streams == 0 : row == 0);
-        const bool edited = a.recent || ignores;
-        if (a.recent)
-            for (int i = tid; i < (count + 31) / 32; i += kThreads) bitmap[i] = 0;
+        groups = (phase + count + L - 1) / L;
+        edits = a.recent || ignores();
         float most = -INFINITY, least = INFINITY;
-        int nan = 0;
-        auto note = [&](float v) {
+        bool nan = false;
+        auto note = [&](float v) {  // neither extreme takes a NaN
+            nan |= isnan(v);
             most = fmaxf(most, v);
-            if (v > -INFINITY) least = fminf(least, v);
+            least = fminf(least, v == -INFINITY ? INFINITY : v);
         };
-        constexpr int kAhead = 4;
-        for (int g0 = tid; g0 < groups; g0 += kAhead * kThreads) {
-            uint4 raw[kAhead];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int g = g0 + j * kThreads, e = g * L - phase;
-                if (e >= 0 && e + L <= count) raw[j] = *reinterpret_cast<const uint4 *>(x + e);
-            }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int g = g0 + j * kThreads, e = g * L - phase;
-                if (g >= groups) break;
-                float v[L];
-                if (e >= 0 && e + L <= count) {
-                    const T *values = reinterpret_cast<const T *>(&raw[j]);
-#pragma unroll
-                    for (int i = 0; i < L; ++i) v[i] = to_float(values[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < L; ++i)
-                        v[i] = e + i >= 0 && e + i < count ? to_float(x[e + i]) : -INFINITY;
-                }
-                if (!edited) {
-#pragma unroll
-                    for (int i = 0; i < L; ++i) {
-                        v[i] = clean(v[i], nan);
-                        note(v[i]);
-                    }
-                }
+        read_groups([&] { if (edits) mark_edits(); }, [&](int g, float(&v)[L]) {
+            if (HELD) {
 #pragma unroll
                 for (int i = 0; i < L; i += 4)
                     *reinterpret_cast<float4 *>(buf + g * L + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                if (edits) {  // what is penalised or ignored is held as it came, and edited below
+                    const uint32_t marks = bits_of(penalised, g) | bits_of(ignored, g);
+                    if (marks) {
+#pragma unroll
+                        for (int i = 0; i < L; ++i)
+                            if (marks >> i & 1) v[i] = -INFINITY;
+                    }
+                }
+            } else if (edits) {
+                edit(v, g);
             }
-        }
-        __syncthreads();
-        if (edited) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) note(v[i]);
+        });
+        if (HELD && edits) {
+            __syncthreads();
             float *const mine = buf + phase;
             if (a.recent)
                 for (int64_t j = tid; j < a.recent_len; j += kThreads) {
-                    const int64_t id = a.recent[row * a.recent_len + j], at_id = id - start;
-                    if (id < 0 || id >= a.limit || at_id < 0 || at_id >= count) continue;
-                    const uint32_t bit = 1u << (at_id & 31);
-                    if (!(atomicOr(&bitmap[at_id >> 5], bit) & bit)) mine[at_id] = __fdiv_rn(mine[at_id], a.penalty);
+                    const int64_t id = a.recent[row * a.recent_len + j], e = id - start;
+                    if (id < 0 || id >= a.limit || e < 0 || e >= count) continue;
+                    const uint32_t bit = 1u << (e & 31);
+                    if ((ignored[e >> 5] & bit) || !(atomicAnd(&penalised[e >> 5], ~bit) & bit)) continue;  // once an id
+                    mine[e] = penalty_of(mine[e], a.penalty);
+                    note(mine[e]);
                 }
-            __syncthreads();
-            if (ignores)
+            if (ignores())
                 for (int64_t j = tid; j < a.n_ignore; j += kThreads) {
-                    const int64_t at_id = a.ignore[j] - start;
-                    if (at_id >= 0 && at_id < count) mine[at_id] = -INFINITY;
+                    const int64_t e = a.ignore[j] - start;
+                    if (e >= 0 && e < count) mine[e] = -INFINITY;
                 }
-            __syncthreads();
-            for (int g = tid; g < quads; g += kThreads) {
-                float4 &q = reinterpret_cast<float4 *>(buf)[g];
-                q = make_float4(clean(q.x, nan), clean(q.y, nan), clean(q.z, nan), clean(q.w, nan));
-                note(q.x), note(q.y), note(q.z), note(q.w);
-            }
         }
+        thread_top = most;
         const uint32_t most_key = __reduce_max_sync(0xffffffffu, key_of(most));
         const uint32_t least_key = __reduce_min_sync(0xffffffffu, key_of(least));
         nan = __any_sync(0xffffffffu, nan);
@@ -317,128 +430,254 @@ class Row {
         lowest = value_of(least);
     }
 
+    // This row's settings (loaded ahead of the row).
+    __device__ void ask() {
+        temperature = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
+        top_k = a.top_k_rows ? a.top_k_rows[row] : a.top_k;
+        top_p = a.top_p_rows ? a.top_p_rows[row] : a.top_p;
+        min_p = a.min_p_rows ? a.min_p_rows[row] : a.min_p;
+        uniform = a.uniforms[row];
+    }
+
     __device__ void settings() {
         bad = false;
-        float temperature = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
         if (!(temperature >= 0.0f) || isinf(temperature)) bad = true, temperature = 0.0f;
-        top_k = a.top_k_rows ? a.top_k_rows[row] : a.top_k;
         if (top_k < 0) bad = true, top_k = 0;
         if (top_k == 0 || top_k > a.vocab) top_k = a.vocab;
-        top_p = a.top_p_rows ? a.top_p_rows[row] : a.top_p;
         if (!(top_p >= 0.0f && top_p <= 1.0f)) bad = true, top_p = top_p < 0.0f ? 0.0f : 1.0f;
-        min_p = a.min_p_rows ? a.min_p_rows[row] : a.min_p;
         if (!(min_p >= 0.0f && min_p <= 1.0f)) bad = true, min_p = min_p > 1.0f ? 1.0f : 0.0f;
-        uniform = a.uniforms[row];
         if (!(uniform >= 0.0f && uniform < 1.0f)) bad = true, uniform = uniform >= 1.0f ? 1.0f : 0.0f;
         if (temperature == 0.0f) top_k = 1;
-        scale = temperature > 0.0f ? 1.4426950408889634074 / static_cast<double>(temperature) : 0.0;
-        if (top == INFINITY) {  // +inf alone has weight: as 0 among -inf
-            for (int g = tid; g < quads; g += kThreads) {
-                float4 &q = reinterpret_cast<float4 *>(buf)[g];
-                q.x = q.x == top ? 0.0f : -INFINITY, q.y = q.y == top ? 0.0f : -INFINITY;
-                q.z = q.z == top ? 0.0f : -INFINITY, q.w = q.w == top ? 0.0f : -INFINITY;
-            }
+        scale = temperature > 0.0f ? kSteps * 1.4426950408889634074 / static_cast<double>(temperature) : 0.0;
+        infinite = top == INFINITY;  // +inf alone has weight: as 0 among -inf
+        if (infinite) {
             top = lowest = 0.0f;
-            __syncthreads();
+            thread_top = thread_top == INFINITY ? 0.0f : -INFINITY;
         }
         // Half differences, so that none overflows.  The slices reach to the lowest logit, or to 31.9 T below the top,
         // where weights are below 2^-45 and round to nothing.
         half_top = 0.5f * top;
         wide_top = top;
-        const float reach = fminf(__fmaf_rn(-0.5f, lowest, half_top), 15.95f * temperature);
-        slices = fminf(__fdiv_rn(static_cast<float>(kBins - 1), reach), FLT_MAX);
+        reach = fminf(__fmaf_rn(-0.5f, lowest, half_top), 15.95f * temperature);
     }
 
-    // Slice of a logit: never smaller for a smaller logit; kBins and above where there is no weight (-inf among it).
-    // The sum with 2^23 leaves the nearest integer in the low bits.
+    // Slice of a logit: never smaller for a smaller logit; `bins` and above where there is no weight (-inf among it)
+    // and for NaN.  The sum with 2^23 leaves the nearest integer in the low bits.
     __device__ uint32_t bin_of(float v) const {
         const float d = __fmaf_rn(-0.5f, v, half_top);
         return __float_as_uint(__fmaf_rn(d, slices, 8388608.0f)) - 0x4b000000u;
     }
-    __device__ bool within(float v, int index) const {
-        return v > limit_value || (v == limit_value && index <= limit_index);
+    // A value below every logit of the slices up to `bin`: the lower edge, moved until it lies outside them.
+    __device__ float below(uint32_t bin) const {
+        const float width = __fdiv_rn(2.0f, slices);
+        for (float past = 1.0f; past < 100.0f; past *= 4.0f) {
+            const float v = __fmaf_rn(-(static_cast<float>(bin) + past), width, top);
+            if (bin_of(v) > bin) return v;
+        }
+        const float next = value_of(key_of(top) - 1);
+        return bin_of(next) > bin ? next : -INFINITY;
     }
-    __device__ u64 weight(float v) const { return weight_of(v, wide_top, scale); }
+    // A value that no logit of the slices from `bin` on lies above.
+    __device__ float above(uint32_t bin) const {
+        const float width = __fdiv_rn(2.0f, slices);
+        for (uint32_t past = 1; past < min(bin, 100u); past *= 4) {
+            const float v = __fmaf_rn(-static_cast<float>(bin - past), width, top);
+            if (bin_of(v) < bin) return v;
+        }
+        return INFINITY;
+    }
+    __device__ bool within(float v, int index) const {
+        return !limited || v > limit_value || (v == limit_value && index <= limit_index);
+    }
+    __device__ u64 weight(float v) const { return weight_of(v, wide_top, scale, sh.powers); }
 
-    // f(logits, slices, index of the first) for this CTA's tokens by fours; a token without weight, or beyond the
-    // limit of top-k, has a slice of kBins or above.
+    // f(logits, index of the first) for this CTA's tokens by fours.
     template <typename F>
     __device__ void for_fours(F f) {
-        for (int g = tid; g < quads; g += kThreads) {
-            const float4 q = reinterpret_cast<const float4 *>(buf)[g];
-            const float v[4] = {q.x, q.y, q.z, q.w};
-            const int first = start + 4 * g - phase;
+        auto four = [&](float(&v)[4], int first) {
+            if (infinite) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = v[i] == INFINITY ? 0.0f : -INFINITY;
+            }
+            f(v, first);
+        };
+        if constexpr (HELD) {
+            const int quads = groups * L / 4;
+            for (int g = tid; g < quads; g += kThreads) {
+                const float4 q = reinterpret_cast<const float4 *>(buf)[g];
+                float v[4] = {q.x, q.y, q.z, q.w};
+                four(v, start + 4 * g - phase);
+            }
+        } else {
+            read_groups([] {}, [&](int g, float(&group)[L]) {
+                if (edits) edit(group, g);
+#pragma unroll
+                for (int i = 0; i < L; i += 4) {
+                    float v[4] = {group[i], group[i + 1], group[i + 2], group[i + 3]};
+                    four(v, start + g * L - phase + i);
+                }
+            });
+        }
+    }
+    // f(logits, slices) for this CTA's tokens by fours; a token without weight, or beyond the limit of top-k, has a
+    // slice of `bins` or above.
+    template <typename F>
+    __device__ void for_slices(F f) {
+        for_fours([&](const float(&v)[4], int first) {
             uint32_t bin[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) bin[i] = bin_of(v[i]);
             if (limited) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (!within(v[i], first + i)) bin[i] = kBins;
+                    if (!within(v[i], first + i)) bin[i] = bins;
             }
-            f(v, bin, first);
-        }
+            f(v, bin);
+        });
     }
 
     // ---- histograms ----------------------------------------------------------------------------------------
     __device__ void add(uint32_t bin, u64 w) {
+#ifdef ADD64
+        atomicAdd(reinterpret_cast<u64 *>(lo) + bin, w);
+        return;
+#endif
         const uint32_t low = static_cast<uint32_t>(w);
         const uint32_t old = atomicAdd(&lo[bin], low);
         const uint32_t high = static_cast<uint32_t>(w >> 32) + (old + low < old);
         if (high) atomicAdd(&hi[bin], high);
     }
 
-    // Running sums of the cluster's histogram, in the first CTA: scan[bin] = what lies before it.
+    __device__ void add4(const uint32_t (&bin)[4], const u64 (&w)[4]) {
+#ifdef ADD64
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (bin[i] < bins) atomicAdd(reinterpret_cast<u64 *>(lo) + bin[i], w[i]);
+#else
+        uint32_t old[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (bin[i] < bins) old[i] = atomicAdd(&lo[bin[i]], static_cast<uint32_t>(w[i]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t high = static_cast<uint32_t>(w[i] >> 32) + (old[i] + static_cast<uint32_t>(w[i]) < old[i]);
+            if (bin[i] < bins && high) atomicAdd(&hi[bin[i]], high);
+        }
+#endif
+    }
+
+    // Running sums of the cluster's histogram, in the first CTA: a slice's words = what lies before it.
     __device__ void running_sums() {
         sync_all();
         if (CLUSTER) {
-            const int share = kBins / ctas;
-            for (int i = tid; i < share; i += kThreads) {
-                const int bin = rank * share + i;
-                u64 sum = 0;
-                for (int c = 0; c < ctas; ++c)
-                    sum += (static_cast<u64>(*at(&hi[bin], c)) << 32) + *at(&lo[bin], c);
-                *at(&scan[bin], 0) = sum;
+            constexpr int kMost = kBins / 2 / kThreads;
+            const int share = bins / ctas;
+            u64 sum[kMost];
+#pragma unroll
+            for (int i = 0; i < kMost; ++i) {
+                const int bin = rank * share + i * kThreads + tid;
+                sum[i] = 0;
+                if (i * kThreads + tid < share) {
+#pragma unroll
+                    for (int c = 0; c < kMaxCluster; ++c) {
+                        const int from = min(c, ctas - 1);  // every load unconditional: all are on their way at once
+                        const u64 part = (static_cast<u64>(*at(&hi[bin], from)) << 32) + *at(&lo[bin], from);
+                        sum[i] += c < ctas ? part : 0;
+                    }
+                }
+            }
+            sync_all();
+#pragma unroll
+            for (int i = 0; i < kMost; ++i) {
+                const int bin = rank * share + i * kThreads + tid;
+                if (i * kThreads + tid < share) {
+                    *at(&lo[bin], 0) = static_cast<uint32_t>(sum[i]);
+                    *at(&hi[bin], 0) = static_cast<uint32_t>(sum[i] >> 32);
+                }
             }
             sync_all();
         }
         if (!leader()) return;
-        constexpr int kEach = kBins / kThreads;
-        u64 own[kEach], sum = 0;
+        if (bins == kBins)
+            add_up<kBins / kThreads>();
+        else
+            add_up<kCountBins / kThreads>();
+    }
+
+    // A thread's N neighbouring sums.
+    template <int N>
+    __device__ void sums_of(u64 (&sum)[N]) const {
+        if constexpr (N % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int bin = tid * kEach + i;
-            own[i] = CLUSTER ? scan[bin] : (static_cast<u64>(hi[bin]) << 32) + lo[bin];
-            sum += own[i];
+            for (int i = 0; i < N; i += 4) {
+                const uint4 l = *reinterpret_cast<const uint4 *>(lo + tid * N + i);
+                const uint4 h = *reinterpret_cast<const uint4 *>(hi + tid * N + i);
+                sum[i] = (static_cast<u64>(h.x) << 32) | l.x, sum[i + 1] = (static_cast<u64>(h.y) << 32) | l.y;
+                sum[i + 2] = (static_cast<u64>(h.z) << 32) | l.z, sum[i + 3] = (static_cast<u64>(h.w) << 32) | l.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] = (static_cast<u64>(hi[tid * N + i]) << 32) | lo[tid * N + i];
         }
-        u64 all;
-        u64 before = sum_before(sum, all);
+    }
+    template <int N>
+    __device__ void add_up() {
+        u64 own[N], sum = 0, all;
+        sums_of(own);
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            scan[tid * kEach + i] = before;
+        for (int i = 0; i < N; ++i) sum += own[i];
+        u64 before = sum_before(sum, all);
+        uint32_t l[N], h[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            l[i] = static_cast<uint32_t>(before);
+            h[i] = static_cast<uint32_t>(before >> 32);
             before += own[i];
+        }
+        if constexpr (N % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < N; i += 4) {
+                *reinterpret_cast<uint4 *>(lo + tid * N + i) = make_uint4(l[i], l[i + 1], l[i + 2], l[i + 3]);
+                *reinterpret_cast<uint4 *>(hi + tid * N + i) = make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) lo[tid * N + i] = l[i], hi[tid * N + i] = h[i];
         }
         if (tid == 0) sh.total = all;
         __syncthreads();
     }
 
     // The slice that `target` (below the total; the first CTA's) falls into, told to every CTA.
+    template <int N>
+    __device__ void find(u64 target) {
+        u64 sum[N];
+        sums_of(sum);
+        const u64 next = tid + 1 < kThreads ? (static_cast<u64>(hi[(tid + 1) * N]) << 32) | lo[(tid + 1) * N] : sh.total;
+        if (sum[0] > target || target >= next) return;
+        int bin = tid * N;
+        u64 before = sum[0], upto = next;
+#pragma unroll
+        for (int i = 1; i < N; ++i) {
+            if (sum[i] <= target)
+                bin = tid * N + i, before = sum[i];
+            else
+                upto = min(upto, sum[i]);
+        }
+        for (int c = 0; c < ctas; ++c) {
+            Shared &to = *at(&sh, c);
+            to.bin = bin;
+            to.before = before;
+            to.upto = upto;
+            to.target = target;
+        }
+    }
     __device__ void locate(u64 target) {
         if (leader()) {
-            constexpr int kEach = kBins / kThreads;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const int bin = tid * kEach + i;
-                const u64 next = bin + 1 < kBins ? scan[bin + 1] : sh.total;
-                if (scan[bin] <= target && target < next)
-                    for (int c = 0; c < ctas; ++c) {
-                        Shared &to = *at(&sh, c);
-                        to.bin = bin;
-                        to.before = scan[bin];
-                        to.upto = next;
-                        to.target = target;
-                    }
-            }
+            if (bins == kBins)
+                find<kBins / kThreads>(target);
+            else
+                find<kCountBins / kThreads>(target);
         }
         sync_all();
     }
@@ -448,48 +687,108 @@ class Row {
     __device__ int collect(uint32_t from, uint32_t to, uint32_t low = 0, uint32_t high = 0xffffffffu) {
         int *const cursor = at(&sh.cursor[searches], 0);
         u64 *const into = at(list, 0);
-        for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int first) {
-            bool any = false;
+        auto member = [&](float v, int index) {
+            const uint32_t key = key_of(v);
+            return bin_of(v) - from <= to - from && key >= low && key <= high && within(v, index);
+        };
+        // all but a few fail the two comparisons
+        const float floor = below(to), ceiling = above(from);
+        if constexpr (HELD) {
+            // a bit a logit of the thread's, then the threads' places by a running sum
+            static_assert(112 * 1024 / sizeof(float) <= 64 * kThreads, "a thread's logits have a bit each");
+            u64 near = 0, mine = 0;
+            int shift = 0;
+            for_fours([&](const float(&v)[4], int) {
+                uint32_t bits = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) any |= bin[i] - from <= to - from;
-            if (!any) return;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t key = key_of(v[i]);
-                if (bin[i] - from > to - from || key < low || key > high) continue;
-                const int place = atomicAdd(cursor, 1);
-                if (place < kList) into[place] = order_of(v[i], first + i);
+                for (int i = 0; i < 4; ++i) bits |= (v[i] > floor && v[i] <= ceiling ? 1u : 0u) << i;
+                near |= static_cast<u64>(bits) << shift;
+                shift += 4;
+            });
+            auto place_of = [&](int bit) { return 4 * (tid + (bit >> 2) * kThreads) + (bit & 3); };
+            auto held = [&](int e) { return infinite ? 0.0f : buf[e]; };
+            for (; near != 0; near &= near - 1) {
+                const int bit = __ffsll(near) - 1, e = place_of(bit);
+                if (member(held(e), start + e - phase)) mine |= 1ull << bit;
             }
-        });
+            u64 all;
+            int place = static_cast<int>(sum_before(static_cast<u64>(__popcll(mine)), all));
+            if (tid == 0) sh.place = atomicAdd(cursor, static_cast<int>(all));
+            __syncthreads();
+            place += sh.place;
+            for (; mine != 0 && place < kList; mine &= mine - 1, ++place) {
+                const int e = place_of(__ffsll(mine) - 1);
+                into[place] = order_of(held(e), start + e - phase);
+            }
+        } else {
+            for_fours([&](const float(&v)[4], int first) {
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) any |= v[i] > floor && v[i] <= ceiling;
+                if (!any) return;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!member(v[i], first + i)) continue;
+                    const int place = atomicAdd(cursor, 1);
+                    if (place < kList) into[place] = order_of(v[i], first + i);
+                }
+            });
+        }
         sync_all();
         ++searches;
         return *cursor;
     }
 
-    // First CTA: the n listed tokens in order, one a thread (all ones behind them).  A bitonic network: strides below a
-    // warp by shuffles, the others through two arrays in turn.
+    // First CTA: the n listed tokens in order, one a thread (all ones behind them).  Up to a warp's: a bitonic network.
+    // More: slices of the list's own range, each token's place is the slice's start and its rank in the slice (few
+    // tokens, unless they are equal).  The histogram is not touched.
     __device__ u64 sorted(int n) {
         u64 mine = tid < n ? list[tid] : ~0ull;
-        u64 *area = list_own, *next = list;
-        __syncthreads();
-        for (int size = 2; size < 2 * n; size <<= 1)
-            for (int stride = size >> 1; stride > 0; stride >>= 1) {
-                u64 other;
-                if (stride >= 32) {
-                    area[tid] = mine;
-                    __syncthreads();
-                    other = area[tid ^ stride];
-                    u64 *const t = area;
-                    area = next;
-                    next = t;
-                } else {
-                    other = __shfl_xor_sync(0xffffffffu, mine, stride);
-                }
-                const bool smaller = ((tid & stride) == 0) == ((tid & size) == 0);
-                if ((other < mine) == smaller) mine = other;
+        if (n <= 32) {
+            if (tid < 32) {
+#pragma unroll
+                for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+                    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+                        const u64 other = __shfl_xor_sync(0xffffffffu, mine, stride);
+                        const bool smaller = ((tid & stride) == 0) == ((tid & size) == 0);
+                        if ((other < mine) == smaller) mine = other;
+                    }
             }
+            return mine;
+        }
+        const uint32_t key = static_cast<uint32_t>(mine >> 32);  // ascending in the order
+        const uint32_t first = __reduce_min_sync(0xffffffffu, key);
+        const uint32_t last = __reduce_max_sync(0xffffffffu, tid < n ? key : 0u);
+        if (tid == 0) sh.block_least = 0xffffffffu, sh.block_most = 0u;
+        sh.places[tid] = 0;
         __syncthreads();
-        return mine;
+        if ((tid & 31) == 0) atomicMin(&sh.block_least, first), atomicMax(&sh.block_most, last);
+        __syncthreads();
+        const float half_first = 0.5f * value_of(~sh.block_least);
+        const float per_unit = fminf(__fdiv_rn(static_cast<float>(kThreads - 1),
+                                               __fmaf_rn(-0.5f, value_of(~sh.block_most), half_first)), FLT_MAX);
+        const float d = __fmaf_rn(-0.5f, value_of(~key), half_first);
+        const int part = tid < n ? min(kThreads - 1, static_cast<int>(d * per_unit)) : 0;
+        if (tid < n) atomicAdd(&sh.places[part], 1);
+        __syncthreads();
+        const int own = sh.places[tid];
+        u64 all;
+        const int before = static_cast<int>(sum_before(static_cast<u64>(own), all));
+        sh.places[tid] = before;
+        sh.ends[tid] = before;
+        __syncthreads();
+        if (tid < n) spare[atomicAdd(&sh.ends[part], 1)] = mine;
+        __syncthreads();
+        int place = 0;
+        if (tid < n) {
+            const int from = sh.places[part], to = sh.ends[part];
+            place = from;
+            for (int i = from; i < to; ++i) place += spare[i] < mine;
+            list[place] = mine;
+        }
+        __syncthreads();
+        return tid < n ? list[tid] : ~0ull;
     }
 
     // Running sum over the CTA's threads (what lies before this one); `all`: the whole.
@@ -546,9 +845,8 @@ class Row {
             // keys of the slice that is left
             uint32_t most = 0, least = 0xffffffffu, group = 0;
             if (tid == 0) sh.block_most = 0, sh.block_least = 0xffffffffu;
-            clear_bins();
             __syncthreads();
-            for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int) {
+            for_slices([&](const float(&v)[4], const uint32_t(&bin)[4]) {
                 for (int i = 0; i < 4; ++i)
                     if (member(v[i], bin[i])) {
                         most = max(most, key_of(v[i])), least = min(least, key_of(v[i]));
@@ -588,8 +886,9 @@ class Row {
                 return false;
             }
             int shift = 0;
-            while (((most - least) >> shift) >= kBins) ++shift;
-            for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int) {
+            while (((most - least) >> shift) >= static_cast<uint32_t>(bins)) ++shift;
+            clear();
+            for_slices([&](const float(&v)[4], const uint32_t(&bin)[4]) {
                 for (int i = 0; i < 4; ++i)
                     if (member(v[i], bin[i])) add((most - key_of(v[i])) >> shift, by_weight ? weight(v[i]) : 1);
             });
@@ -606,13 +905,24 @@ class Row {
         }
     }
 
+    // One of this CTA's logits as the order sees it.
+    __device__ float logit(int i) const {
+        float v = HELD ? buf[phase + i] : to_float(x[i]);
+        if (!HELD && edits) {
+            const uint32_t bit = 1u << (i & 31);
+            if (penalised[i >> 5] & bit) v = penalty_of(v, a.penalty);
+            if (ignored[i >> 5] & bit) v = -INFINITY;
+        }
+        return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
+    }
+
     // Index of this CTA's n-th (from 0) token with that logit: in the thread that holds it, -1 in the others.
     __device__ int nth(float value, uint32_t n) {
         uint32_t before = 0;
         int found = -1;
         for (int i0 = 0; i0 < count && before <= n; i0 += kThreads) {
             const int i = i0 + tid;
-            const bool is = i < count && buf[phase + i] == value;
+            const bool is = i < count && logit(i) == value;
             const uint32_t vote = __ballot_sync(0xffffffffu, is);
             __syncthreads();
             if ((tid & 31) == 0) sh.warp_counts[tid >> 5] = __popc(vote);
@@ -632,26 +942,44 @@ class Row {
         return static_cast<u64>(ceil(static_cast<double>(min_p) * 17592186044416.0));  // 2^44
     }
 
-    // The histogram of weights and its running sums; what min-p leaves of them to the first CTA.
-    __device__ void weigh() {
-        const u64 least = least_weight();
-        u64 passing = 0;
-        for_fours([&](const float(&v)[4], const uint32_t(&bin)[4], int) {
-            if (bin[0] >= kBins && bin[1] >= kBins && bin[2] >= kBins && bin[3] >= kBins) return;
-            u64 w[4];
+    // The slice that holds the k-th largest of the threads' largest logits: k tokens or more lie up to it, and few more
+    // where k is well below the number of threads.  `bins` where the threads have fewer than k.
+    __device__ int enough_for(int64_t k) {
+        const uint32_t bin = bin_of(thread_top);
+        if (bin < bins) atomicAdd(&lo[bin], 1u);
+        running_sums();
+        locate(leader() ? min(static_cast<u64>(k), sh.total) - 1 : 0);
+        return sh.target + 1 == static_cast<u64>(k) ? sh.bin : bins;
+    }
+
+    // The histogram of counts, or of weights (and then what min-p leaves of them, to the first CTA), and its running
+    // sums.
+    __device__ void histogram(bool of_weights) {
+        if (!of_weights) {
+            for_slices([&](const float(&)[4], const uint32_t(&bin)[4]) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = weight(bin[i] < kBins ? v[i] : top);
+                for (int i = 0; i < 4; ++i)
+                    if (bin[i] < bins) atomicAdd(&lo[bin[i]], 1u);
+            });
+        } else {
+            const u64 least = least_weight();
+            const bool counted = min_p > 0.0f;
+            u64 passing = 0;
+            for_slices([&](const float(&v)[4], const uint32_t(&bin)[4]) {
+                if (min(min(bin[0], bin[1]), min(bin[2], bin[3])) >= bins) return;
+                u64 w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (bin[i] < kBins) {
-                    add(bin[i], w[i]);
-                    if (w[i] >= least) passing += w[i];
-                }
-        });
-        if (min_p > 0.0f) {
-            u64 all;
-            sum_before(passing, all);
-            if (tid == 0) at(&sh, 0)->passing[rank] = all;
+                for (int i = 0; i < 4; ++i) w[i] = weight(bin[i] < bins ? v[i] : top);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (counted && bin[i] < bins && w[i] >= least) passing += w[i];
+                add4(bin, w);
+            });
+            if (min_p > 0.0f) {
+                u64 all;
+                sum_before(passing, all);
+                if (tid == 0) at(&sh, 0)->passing[rank] = all;
+            }
         }
         running_sums();
     }
@@ -689,59 +1017,71 @@ class Row {
     }
 
     __device__ void sample() {
+        enum { kTopK, kTopP, kDraw } stage = top_k < a.vocab ? kTopK : top_p < 1.0f ? kTopP : kDraw;
+        bool fresh = true;  // the stage needs a histogram of its own
+        u64 kept = 0;       // first CTA: weight that is kept
+        new_bins(stage == kTopK ? kCountBins : kBins);
         if (a.vocab <= kList) {
-            const int n = collect(0, kBins - 1);
+            const int n = collect(0, bins - 1);
             if (leader()) sample_list(n);
             return;
         }
-        if (top_k < a.vocab) {
-            for_fours([&](const float(&)[4], const uint32_t(&bin)[4], int) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (bin[i] < kBins) atomicAdd(&lo[bin[i]], 1u);
-            });
-            running_sums();
-            locate(leader() ? min(static_cast<u64>(top_k), sh.total) - 1 : 0);
-            // The k-th token's slice, or the last one with a token.  Few enough up to it: the first CTA has them all.
-            if (sh.upto <= kList) {
+        if (stage == kTopK && top_k <= kList) {
+            const int slice = enough_for(top_k);
+            if (slice < bins) {
+                const int n = collect(0, slice);
+                if (n <= kList) {
+                    if (leader()) sample_list(n);
+                    return;
+                }
+            }
+            sync_all();  // the histogram has been read
+            new_bins(kCountBins);
+        }
+        for (;;) {
+            if (fresh) {
+                histogram(stage != kTopK);
+                if (stage != kTopK && kept == 0) kept = leader() ? sh.total : 0;
+            }
+            if (stage == kDraw && min_p > 0.0f && leader()) {
+                u64 passing = 0;
+                for (int c = 0; c < ctas; ++c) passing += sh.passing[c];
+                kept = min(kept, passing);
+            }
+            u64 target = 0;
+            if (leader())
+                target = stage == kTopK ? min(static_cast<u64>(top_k), sh.total) - 1
+                         : stage == kTopP ? nucleus(kept)
+                                          : drawn(kept);
+            locate(target);
+            // Few tokens up to the k-th one's slice (or the last slice with a token): the first CTA has them all.
+            if (stage == kTopK && sh.upto <= kList) {
                 const int n = collect(0, sh.bin);
                 if (leader()) sample_list(n);
                 return;
             }
-            if (sh.target + 1 == static_cast<u64>(top_k)) {
-                search_slice(false);
-                if (CLUSTER) {
-                    if (leader() && tid > 0 && tid < ctas) at(&sh, tid)->found = sh.found;
-                    sync_all();
+            bool whole = false;
+            if (stage != kTopK || sh.target + 1 == static_cast<u64>(top_k)) {
+                whole = search_slice(stage != kTopK);
+                if (stage == kTopK) {
+                    if (CLUSTER) {
+                        if (leader() && tid > 0 && tid < ctas) at(&sh, tid)->found = sh.found;
+                        sync_all();
+                    }
+                    limited = true;
+                    limit_value = value_in(sh.found.order);
+                    limit_index = index_in(sh.found.order);
                 }
-                limited = true;
-                limit_value = value_in(sh.found.order);
-                limit_index = index_in(sh.found.order);
             }
-            sync_all();  // the histograms have been read
-            clear_bins();
-            __syncthreads();
-        }
-        weigh();
-        u64 kept = leader() ? sh.total : 0;
-        if (top_p < 1.0f) {
-            locate(leader() ? nucleus(kept) : 0);
-            const bool whole = search_slice(true);
-            kept = leader() ? sh.found.before + sh.found.own : 0;
-            if (!whole) {
-                sync_all();
-                clear_bins();
-                __syncthreads();
-                weigh();
+            if (stage == kDraw) break;
+            if (stage == kTopP) kept = leader() ? sh.found.before + sh.found.own : 0;
+            fresh = stage == kTopK || !whole;
+            stage = stage == kTopK && top_p < 1.0f ? kTopP : kDraw;
+            if (fresh) {
+                sync_all();  // the histograms have been read
+                new_bins(kBins);
             }
         }
-        if (min_p > 0.0f && leader()) {
-            u64 passing = 0;
-            for (int c = 0; c < ctas; ++c) passing += sh.passing[c];
-            kept = min(kept, passing);
-        }
-        locate(leader() ? drawn(kept) : 0);
-        search_slice(true);
         finish(index_in(sh.found.order), sh.found.own, kept);
     }
 
@@ -757,38 +1097,40 @@ class Row {
     }
 };
 
-template <typename T, bool CLUSTER>
+template <typename T, bool CLUSTER, bool HELD>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ Shared shared;
-    Row<T, CLUSTER> row(a, shared, dynamic);
+    Row<T, CLUSTER, HELD> row(a, shared, dynamic);
     row.run(CLUSTER ? blockIdx.x / cg::this_cluster().num_blocks() : blockIdx.x);
 }
 
+#ifndef MINV
+#define MINV 4096
+#endif
 template <typename T>
 int launch_sample(SampleArgs &a, const char *what, cudaStream_t stream) {
     constexpr int L = 16 / sizeof(T);
-    auto chunk_of = [&](int ctas) { return static_cast<int>((a.vocab + ctas - 1) / ctas + 7) / 8 * 8; };
-    auto smem_of = [&](int ctas) {
-        const size_t slots = (chunk_of(ctas) + 2 * L + 3) / 4 * 4, words = a.recent ? (chunk_of(ctas) + 31) / 32 : 0;
-        return slots * sizeof(float) + 2 * kBins * sizeof(uint32_t) + (kBins + 2 * kList) * sizeof(u64) + words * 4;
-    };
-    // As many CTAs a row as leave every CTA work, while the SMs (two CTAs each) are not filled by the rows.
+    // As many CTAs a row as the SMs (two CTAs each) take at once, each with a share that is worth it.
     int ctas = 1;
-    while (ctas < kMaxCluster && (smem_of(ctas) > 110 * 1024 ||
-                                  (a.rows * ctas * 2 <= 2LL * sm_count() && a.vocab / ctas >= 4096)))
-        ctas *= 2;
-    a.chunk = chunk_of(ctas);
+    while (ctas < kMaxCluster && a.rows * ctas * 2 <= 2LL * sm_count() && a.vocab / ctas >= 2 * MINV) ctas *= 2;
+    a.chunk = static_cast<int>((a.vocab + ctas - 1) / ctas + 7) / 8 * 8;
+    a.words = a.recent || a.ignore ? (a.chunk + 31) / 32 + 2 : 0;
+    // A share that leaves room for two CTAs an SM is held in shared memory, a longer one read again from L2.
+    const size_t rest = 2 * kBins * sizeof(uint32_t) + 2 * kList * sizeof(u64);
     a.slots = (a.chunk + 2 * L + 3) / 4 * 4;
+    const bool held = rest + a.slots * sizeof(float) + sizeof(Shared) <= 112 * 1024;
+    if (!held) a.slots = kRing * kThreads * 4;
     if (a.rows * ctas > 0x7fffffff)
         return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": too many rows for one call");
     // Above 48 KB with the static part the kernel has to opt in, which resident_ctas does from the dynamic part alone.
-    size_t smem = smem_of(ctas);
+    size_t smem = rest + a.slots * sizeof(float) + (held ? 0 : 2 * a.words * sizeof(uint32_t));
     if (smem + sizeof(Shared) > 48 * 1024) smem = std::max<size_t>(smem, 48 * 1024 + 16);
-    const void *kernel = ctas > 1 ? reinterpret_cast<const void *>(sample_kernel<T, true>)
-                                  : reinterpret_cast<const void *>(sample_kernel<T, false>);
+    auto *const kernel = ctas > 1 ? (held ? sample_kernel<T, true, true> : sample_kernel<T, true, false>)
+                                  : (held ? sample_kernel<T, false, true> : sample_kernel<T, false, false>);
     int per_sm = 0;
-    if (resident_ctas(kernel, kThreads, smem, &per_sm) != cudaSuccess) return check_launch(what);
+    if (resident_ctas(reinterpret_cast<const void *>(kernel), kThreads, smem, &per_sm) != cudaSuccess)
+        return check_launch(what);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.rows * ctas));
     cfg.blockDim = dim3(kThreads);
@@ -800,9 +1142,7 @@ int launch_sample(SampleArgs &a, const char *what, cudaStream_t stream) {
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = ctas > 1 ? 1 : 0;
-    const cudaError_t err = ctas > 1 ? cudaLaunchKernelEx(&cfg, sample_kernel<T, true>, a)
-                                     : cudaLaunchKernelEx(&cfg, sample_kernel<T, false>, a);
-    (void)err;
+    (void)cudaLaunchKernelEx(&cfg, kernel, a);
     return check_launch(what);
 }
 
@@ -851,7 +1191,7 @@ LEVO_OPS_API int levo_sample_tokens(const levo_sampling *sampling, levo_stream_t
                        s.top_k_rows, s.temperature, s.top_p, s.min_p, s.penalty, s.top_k,
                        s.recent_len > 0 ? s.recent : nullptr, s.recent_len, limit,
                        s.n_ignore > 0 ? s.ignore : nullptr, s.n_ignore, s.streams, s.tokens_out, s.logprob_out,
-                       s.status, 0, 0};
+                       s.status, 0, 0, 0};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (s.dtype == LEVO_DTYPE_F32) return launch_sample<float>(a, w, st);
     if (s.dtype == LEVO_DTYPE_F16) return launch_sample<__half>(a, w, st);
