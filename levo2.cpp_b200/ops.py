@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import pathlib
+import struct
 from typing import Optional
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "liblevo_b200.so"
@@ -237,10 +238,10 @@ SIGNATURES = {
     "levo_gated_layernorm_modulate_f32": (_INT, [_P, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _F, _P]),
     "levo_vae_decode_noalloc_f32": (_INT, [ctypes.POINTER(Topology), _P, _P, _I64, _P, CONV_FN, _P, _U32, _P]),
     "levo_greedy_tokens_f32": (_INT, [_P, _I64, _I64, _I64, _P, _I64, _F, _I64, _P, _I64, _P, _P, _P]),
-    "levo_rope_qk": (_INT, [ctypes.POINTER(Rope), _P]),
+    "levo_rope_qk": (_INT, [_P, _P]),
     "levo_rope_theta_host": (_INT, [_P, _I64, _D, _I32, _D, _D, _D, _D]),
-    "levo_rope_append_kv": (_INT, [ctypes.POINTER(RopeAppend), _P]),
-    "levo_sample_tokens": (_INT, [ctypes.POINTER(Sampling), _P]),
+    "levo_rope_append_kv": (_INT, [_P, _P]),
+    "levo_sample_tokens": (_INT, [_P, _P]),
     "levo_latent_to_vae_f32": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
     "levo_latent_normalize_f32": (_INT, [_P, _P, _P, _I64, _I64, _P, _P, _P]),
     "levo_assemble_windows_f32": (_INT, [_P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I32, _P, _P]),
@@ -592,32 +593,56 @@ def greedy_tokens_t(logits, recent=None, penalty=1.0, penalty_limit=0, ignore=No
 # token step: rotary positions, KV append, sampling
 # ---------------------------------------------------------------------------
 
-def _dtype_of(t) -> int:
+# These calls run once a token and layer, so the binding's own time counts: settled lookups, the arguments packed
+# in one step (the layouts of the structures above), plain device indexes and the raw stream handle.
+_PACK_ROPE = struct.Struct("@PPqqqqqqq" "PPqqqqqqq" "qqqq" "PP" "qq" "q" "iIf4x")
+_PACK_APPEND = struct.Struct(_PACK_ROPE.format + "PPqqqqqqq" "qq" "PPP")
+_PACK_SAMPLING = struct.Struct("@P" "qqq" "PPPPP" "q" "P" "qq" "P" "qq" "PPP" "ffff" "i4x")
+assert (_PACK_ROPE.size, _PACK_APPEND.size, _PACK_SAMPLING.size) == tuple(
+    ctypes.sizeof(c) for c in (Rope, RopeAppend, Sampling))
+_NO_TENSOR = (0, 0, 0, 0, 0, 0, 0, 0, 0)
+_codes: dict = {}
+_torch = _raw_stream = _current_device = None
+
+
+def _bind() -> None:
+    """Settles, on the first of these calls, what every call looks up in torch."""
+    global _torch, _raw_stream, _current_device
     import torch
 
-    code = {torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16}.get(t.dtype)
+    _codes.update({torch.float32: DTYPE_F32, torch.float16: DTYPE_F16, torch.bfloat16: DTYPE_BF16})
+    # handle of a device's current stream, and the current device's index, without the objects around them
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    _torch = torch
+
+
+def _dtype_of(t) -> int:
+    code = _codes.get(t.dtype)
     if code is None:
         raise ValueError("tensors must be float32, float16 or bfloat16")
     return code
 
 
-def _same_device(device, *tensors) -> None:
+def _same_device(index: int, *tensors) -> None:
     for t in tensors:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError("all tensors of a call must lie on one CUDA device")
 
 
-def _launch(call, args, device) -> None:
-    """Calls the library on `device` and its current stream, whatever device is current."""
-    import torch
-
-    if device.type != "cuda":
+def _launch(name: str, args: bytes, index: int) -> None:
+    """Calls the library on device `index` and its current stream, whatever device is current."""
+    if index < 0:
         raise ValueError("levo_b200 ops take CUDA tensors")
-    if torch.cuda.current_device() == device.index:
-        check(call(ctypes.byref(args), _stream(device)))
+    call = getattr(_lib if _lib is not None else lib(), name)
+    if _current_device() == index:
+        code = call(args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            check(call(ctypes.byref(args), _stream(device)))
+        with _torch.cuda.device(index):
+            code = call(args, _raw_stream(index))
+    if code != OK:
+        check(code)
 
 
 def rope_theta(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
@@ -635,36 +660,42 @@ def rope_theta(rotary_dim: int, base: float = 10000.0, scaling: str = "none", fa
     return theta if device is None else theta.to(device)
 
 
-def _rope_tensor(name, x, out, batch, tokens):
-    """RopeTensor of x [batch, tokens, heads, dim] and its output (any outer strides, unit stride in dim)."""
-    if x.dim() != 4 or x.shape[0] != batch or x.shape[1] != tokens:
+def _rope_tensor(name, x, out, batch, tokens, rows, target="output"):
+    """The fields of a levo_rope_tensor: x [batch, tokens, heads, dim] and its output [batch, rows, heads, dim],
+    any outer strides, unit stride in dim."""
+    shape, to = x.shape, out.shape
+    if len(shape) != 4 or shape[0] != batch or shape[1] != tokens:
         raise ValueError(f"{name} must be [batch, tokens, heads, dim], its batch and tokens those of q")
-    if out.dim() != 4 or out.dtype != x.dtype:
-        raise ValueError(f"{name}'s output must be a 4-D tensor of its dtype")
-    xs, os_ = x.stride(), out.stride()
-    if (xs[3] != 1 or os_[3] != 1) and x.shape[3] > 1:
+    if len(to) != 4 or to[0] != batch or to[1] != rows or to[2:] != shape[2:]:
+        raise ValueError(f"the {name} {target} must be [{batch}, {rows}, heads, dim] as {name} is")
+    if out.dtype != x.dtype:
+        raise ValueError(f"the {name} {target} must have the dtype of {name}")
+    s, o = x.stride(), out.stride()
+    if (s[3] != 1 or o[3] != 1) and shape[3] > 1:
         raise ValueError(f"{name} must have unit stride in its last dimension")
-    return RopeTensor(x.data_ptr(), out.data_ptr(), x.shape[2], xs[0], xs[1], xs[2], os_[0], os_[1], os_[2])
+    return x.data_ptr(), out.data_ptr(), shape[2], s[0], s[1], s[2], o[0], o[1], o[2]
 
 
-def _rope_args(q, k, theta, positions, start, flags, magnitude, q_tensor, k_tensor):
-    import torch
-
+def _rope_args(q, theta, positions, start, flags, magnitude):
+    """The fields of a levo_rope behind its tensors."""
+    torch = _torch
+    code = _dtype_of(q)
     if theta.dtype != torch.float64 or theta.dim() != 1 or not theta.is_contiguous():
         raise ValueError("theta must be a contiguous float64 [rotary_dim/2]")
     batch, tokens, _, dim = q.shape
-    ps = (0, 0)
+    where = ps0 = ps1 = 0
     if positions is not None:
         if positions.dtype != torch.int64:
             raise ValueError("positions must be int64")
-        if positions.dim() == 1 and positions.shape[0] == tokens:
-            ps = (0, positions.stride(0))
-        elif positions.dim() == 2 and positions.shape[0] == batch and positions.shape[1] == tokens:
-            ps = positions.stride()
+        shape = positions.shape
+        if len(shape) == 1 and shape[0] == tokens:
+            ps1 = positions.stride(0)
+        elif len(shape) == 2 and shape[0] == batch and shape[1] == tokens:
+            ps0, ps1 = positions.stride()
         else:
             raise ValueError("positions must be [tokens] or [batch, tokens]")
-    return Rope(q_tensor, k_tensor, batch, tokens, dim, 2 * theta.shape[0], theta.data_ptr(), _ptr(positions), ps[0],
-                ps[1], start, _dtype_of(q), flags, magnitude)
+        where = positions.data_ptr()
+    return (batch, tokens, dim, 2 * theta.shape[0], theta.data_ptr(), where, ps0, ps1, start, code, flags, magnitude)
 
 
 def rope_qk_t(q, k, theta, positions=None, *, start=0, interleaved=False, adjoint=False, magnitude=1.0, q_out=None,
@@ -673,24 +704,25 @@ def rope_qk_t(q, k, theta, positions=None, *, start=0, interleaved=False, adjoin
     theta: rope_theta(...) on the device, its pairs the first 2 * len(theta) values of a head; positions int64
     [tokens] or [batch, tokens] (default: start + token).  adjoint=True gives the gradients of q and k from those
     of the outputs.  Any outer strides; an output may be its input."""
-    import torch
-
+    if _torch is None:
+        _bind()
+    torch = _torch
+    if q.dim() != 4:
+        raise ValueError("q must be [batch, tokens, heads, dim]")
     q_out = torch.empty_like(q) if q_out is None else q_out
+    batch, tokens, _, dim = q.shape
+    k_fields = _NO_TENSOR
     if k is not None:
-        k_out = torch.empty_like(k) if k_out is None else k_out
-        if k.dtype != q.dtype or k.shape[-1] != q.shape[-1]:
+        if k.dtype != q.dtype or k.shape[-1] != dim:
             raise ValueError("q and k must share a dtype and a head dimension")
-        if k_out.shape != k.shape:
-            raise ValueError("k_out must have the shape of k")
-    if q.dim() != 4 or q_out.shape != q.shape:
-        raise ValueError("q must be [batch, tokens, heads, dim] and q_out of its shape")
-    _same_device(q.device, k, theta, positions, q_out, k_out)
-    batch, tokens = q.shape[:2]
-    args = _rope_args(q, k, theta, positions, start,
-                      (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_ADJOINT if adjoint else 0), magnitude,
-                      _rope_tensor("q", q, q_out, batch, tokens),
-                      RopeTensor() if k is None else _rope_tensor("k", k, k_out, batch, tokens))
-    _launch(lib().levo_rope_qk, args, q.device)
+        k_out = torch.empty_like(k) if k_out is None else k_out
+        k_fields = _rope_tensor("k", k, k_out, batch, tokens, tokens)
+    args = _rope_args(q, theta, positions, start, (ROPE_INTERLEAVED if interleaved else 0)
+                      | (ROPE_ADJOINT if adjoint else 0), magnitude)
+    index = q.get_device()
+    _same_device(index, k, theta, positions, q_out, k_out)
+    _launch("levo_rope_qk", _PACK_ROPE.pack(*_rope_tensor("q", q, q_out, batch, tokens, tokens), *k_fields, *args),
+            index)
     return q_out, k_out
 
 
@@ -699,32 +731,33 @@ def rope_append_kv_t(q, k, v, theta, k_cache, v_cache, lengths, *, counts=None, 
     """Turns q [batch, tokens, heads, dim] and appends turned k and v to the caches [batch, capacity, kv heads,
     dim]: token s < counts[b] of sequence b goes to row lengths[b] + s (int64 device tensors, not advanced here).
     Returns q_out; APPEND_NO_ROOM / APPEND_BAD_COUNT in the optional status word."""
-    import torch
-
+    if _torch is None:
+        _bind()
+    torch = _torch
+    if q.dim() != 4 or k_cache.dim() != 4 or v_cache.dim() != 4:
+        raise ValueError("q must be [batch, tokens, heads, dim], the caches [batch, capacity, heads, dim]")
     q_out = torch.empty_like(q) if q_out is None else q_out
-    if q.dim() != 4 or q_out.shape != q.shape:
-        raise ValueError("q must be [batch, tokens, heads, dim] and q_out of its shape")
     batch, tokens, _, dim = q.shape
-    for name, x, cache in (("k", k, k_cache), ("v", v, v_cache)):
-        if x.dtype != q.dtype:
-            raise ValueError("q, k and v must share a dtype")
-        if cache.dim() != 4 or cache.shape[0] != batch or x.dim() != 4 or cache.shape[2:] != x.shape[2:]:
-            raise ValueError(f"the {name} cache must be [batch, capacity, heads, dim] as {name} is")
-    if k.shape[3] != dim:
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("q, k and v must share a dtype")
+    if k.shape[-1] != dim:
         raise ValueError("q and k must share a head dimension")
-    if k_cache.shape[1] != v_cache.shape[1]:
+    capacity = k_cache.shape[1]
+    if v_cache.shape[1] != capacity:
         raise ValueError("the caches must share a capacity")
     for name, t in (("lengths", lengths), ("counts", counts)):
-        if t is not None and (t.dtype != torch.int64 or t.shape != (batch,) or not t.is_contiguous()):
+        if t is not None and (t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != batch or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous int64 [batch]")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise ValueError("status must be an int32 tensor")
-    _same_device(q.device, k, v, theta, k_cache, v_cache, lengths, counts, positions, q_out, status)
-    rope = _rope_args(q, k, theta, positions, start, ROPE_INTERLEAVED if interleaved else 0, magnitude,
-                      _rope_tensor("q", q, q_out, batch, tokens), _rope_tensor("k", k, k_cache, batch, tokens))
-    args = RopeAppend(rope, _rope_tensor("v", v, v_cache, batch, tokens), v.shape[3], k_cache.shape[1],
-                      lengths.data_ptr(), _ptr(counts), _ptr(status))
-    _launch(lib().levo_rope_append_kv, args, q.device)
+    args = _rope_args(q, theta, positions, start, ROPE_INTERLEAVED if interleaved else 0, magnitude)
+    index = q.get_device()
+    _same_device(index, k, v, theta, k_cache, v_cache, lengths, counts, positions, q_out, status)
+    v_fields = _rope_tensor("v", v, v_cache, batch, tokens, capacity, "cache")
+    _launch("levo_rope_append_kv", _PACK_APPEND.pack(
+        *_rope_tensor("q", q, q_out, batch, tokens, tokens), *_rope_tensor("k", k, k_cache, batch, tokens, capacity, "cache"),
+        *args, *v_fields, v.shape[3], capacity, lengths.data_ptr(), 0 if counts is None else counts.data_ptr(),
+        0 if status is None else status.data_ptr()), index)
     return q_out
 
 
@@ -733,38 +766,57 @@ def sample_tokens_t(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, mi
     """One token per row of logits [rows, vocab] from uniforms [rows] in [0, 1) (levo_sample_tokens); returns the
     int64 tokens.  temperature, top_p, min_p (float32) and top_k (int64) are numbers or [rows] tensors; logprobs
     (float32 [rows], optional) receives the log of each token's share; SAMPLE_* bits in the optional status word."""
-    import torch
-
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    if _torch is None:
+        _bind()
+    torch = _torch
+    shape = logits.shape
+    if len(shape) != 2 or (shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits must be [rows, vocab] with unit stride in vocab")
-    rows, vocab = logits.shape
-    out = torch.empty(rows, dtype=torch.int64, device=logits.device) if out is None else out
+    rows, vocab = shape
+    code = _dtype_of(logits)
+    index = logits.get_device()
     f32, i64 = torch.float32, torch.int64
-    rowwise = [None, None, None, None]
-    scalar = [temperature, top_k, top_p, min_p]
-    for n, (value, dtype, off) in enumerate(((temperature, f32, 1.0), (top_k, i64, 0), (top_p, f32, 1.0),
-                                             (min_p, f32, 0.0))):
-        if isinstance(value, torch.Tensor):
-            rowwise[n], scalar[n] = value, off
-            if value.dtype != dtype or value.shape != (rows,) or not value.is_contiguous():
-                raise ValueError(f"a per-row setting must be a contiguous {dtype} [rows]")
-    for t, dtype in ((uniforms, f32), (out, i64), (logprobs, f32)):
-        if t is not None and (t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous()):
-            raise ValueError("uniforms and logprobs must be contiguous float32 [rows], out a contiguous int64 [rows]")
-    if recent is not None and (recent.dtype != i64 or recent.dim() != 2 or recent.shape[0] != rows
-                               or not recent.is_contiguous()):
-        raise ValueError("recent must be a contiguous int64 [rows, n]")
-    if ignore is not None and (ignore.dtype != i64 or not ignore.is_contiguous()):
-        raise ValueError("ignore must be a contiguous int64 tensor")
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
-        raise ValueError("status must be an int32 tensor")
-    _same_device(logits.device, uniforms, *rowwise, recent, ignore, logprobs, status, out)
-    args = Sampling(logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, uniforms.data_ptr(),
-                    _ptr(rowwise[0]), _ptr(rowwise[1]), _ptr(rowwise[2]), _ptr(rowwise[3]), scalar[1], _ptr(recent),
-                    0 if recent is None else recent.shape[1], penalty_limit, _ptr(ignore),
-                    0 if ignore is None else ignore.numel(), streams, out.data_ptr(), _ptr(logprobs), _ptr(status),
-                    scalar[0], scalar[2], scalar[3], penalty, _dtype_of(logits))
-    _launch(lib().levo_sample_tokens, args, logits.device)
+    if out is None:
+        out = torch.empty(rows, dtype=i64, device=logits.device)
+
+    def vector(t, dtype, what):
+        """Address of a contiguous [rows] tensor on the logits' device, 0 for None."""
+        if t is None:
+            return 0
+        if t.dtype != dtype or t.dim() != 1 or t.shape[0] != rows or not t.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous {dtype} [rows]")
+        if t.get_device() != index:
+            raise ValueError("all tensors of a call must lie on one CUDA device")
+        return t.data_ptr()
+
+    each_temperature = each_top_k = each_top_p = each_min_p = 0
+    if isinstance(temperature, torch.Tensor):
+        each_temperature, temperature = vector(temperature, f32, "a per-row setting (temperature)"), 1.0
+    if isinstance(top_k, torch.Tensor):
+        each_top_k, top_k = vector(top_k, i64, "a per-row setting (top_k)"), 0
+    if isinstance(top_p, torch.Tensor):
+        each_top_p, top_p = vector(top_p, f32, "a per-row setting (top_p)"), 1.0
+    if isinstance(min_p, torch.Tensor):
+        each_min_p, min_p = vector(min_p, f32, "a per-row setting (min_p)"), 0.0
+    recent_at = recent_len = ignore_at = n_ignore = status_at = 0
+    if recent is not None:
+        if recent.dtype != i64 or recent.dim() != 2 or recent.shape[0] != rows or not recent.is_contiguous():
+            raise ValueError("recent must be a contiguous int64 [rows, n]")
+        recent_at, recent_len = recent.data_ptr(), recent.shape[1]
+    if ignore is not None:
+        if ignore.dtype != i64 or not ignore.is_contiguous():
+            raise ValueError("ignore must be a contiguous int64 tensor")
+        ignore_at, n_ignore = ignore.data_ptr(), ignore.numel()
+    if status is not None:
+        if status.dtype != torch.int32 or status.numel() < 1:
+            raise ValueError("status must be an int32 tensor")
+        status_at = status.data_ptr()
+    _same_device(index, recent, ignore, status)
+    _launch("levo_sample_tokens", _PACK_SAMPLING.pack(
+        logits.data_ptr(), rows, vocab, logits.stride(0) if rows > 1 else vocab, vector(uniforms, f32, "uniforms"),
+        each_temperature, each_top_k, each_top_p, each_min_p, top_k, recent_at, recent_len, penalty_limit, ignore_at,
+        n_ignore, streams, vector(out, i64, "out"), vector(logprobs, f32, "logprobs"), status_at, temperature, top_p,
+        min_p, penalty, code), index)
     return out
 
 
