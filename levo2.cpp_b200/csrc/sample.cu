@@ -3,23 +3,38 @@
 // selection have gone through (the formulas stand at levo_sampling).
 //
 // All three filters keep a prefix of one order (larger logit first, equal logits
-// by index), and the draw is a place in that prefix.  So nothing is sorted: top-k,
-// top-p and the draw are each the search for the one token at which a running
-// count, or a running weight, passes a target:
-//   1. a histogram (of counts, or of weights) over kBins equal slices of the
-//      logits' range below the maximum, and its running sums;
+// by index), and the draw is a place in that prefix.  So the row is not sorted:
+// top-k, top-p and the draw are each the search for the one token at which a
+// running count, or a running weight, passes a target:
+//   1. a histogram (of counts, or of weights) over equal slices of the logits'
+//      range below the maximum, and its running sums;
 //   2. the slice that the target falls into;
 //   3. its tokens, some tens of 16385, in a list; each adds up what lies before it.
 // A slice of more than kList tokens (many equal or close logits) is cut further by
-// the bits of its keys until its tokens are few or all equal.
+// the bits of its keys until its tokens are few or all equal.  Two shortcuts:
+//   - top-k up to kList: the k-th largest of the threads' own largest logits is a
+//     lower bound of the k-th largest, and few tokens lie between (k = 50 of 16385
+//     over 512 threads: about 53 in all).  They are listed and ordered, and the
+//     rest happens in the list;
+//   - top-p and the draw: what top-p keeps is known to a slice before its token is
+//     found, which mostly fixes the draw's slice as well: one pass lists both.
 //
 // Weights are F64 exponentials rounded to multiples of 2^-44 of the largest and
 // summed as 64-bit integers (131072 * 2^44 = 2^61): exact, in any order, so that
-// atomics and the split over CTAs cannot change a result.
+// atomics and the split over CTAs cannot change a result.  F32 sums would put one
+// flat row in some hundreds on another token: a border lies within 1e-7 of one of
+// 1e5 others.
 //
-// A row is held in shared memory as F32 and read from HBM once.  It is split over
-// a cluster of up to 8 CTAs where there are few rows or it is long; the cluster's
-// first CTA merges the histograms, takes the decisions and holds the list.
+// A CTA's share of a row is held in shared memory as F32 and read from HBM once; a
+// share that does not fit beside a second CTA on the SM is read again from L2, by a
+// ring of cp.async copies.  Rows that are few and long are split over a cluster,
+// whose first CTA merges the histograms, takes the decisions and holds the lists.
+//
+// What bounds it: instruction issue, not bytes.  1024 rows of 16385 in F16 (half of
+// them over the whole vocabulary) take 72 us, 5.1 us of HBM time: 48 million warp
+// instructions, 62 % of the issue slots, about 35 a logit for its weight (11 of them
+// F64) and 20 for the load, the slice and the lists.  Small batches are bound by the
+// chain of some ten phases between barriers, 1 to 2 us each for a cluster.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -43,8 +58,11 @@ constexpr int kCountBins = 512;  // and of one of counts
 constexpr int kList = 512;
 static_assert(kList == kThreads, "a listed token a thread");
 constexpr int kMaxCluster = 8;
+// Logits that a cluster's CTA is worth.  Three rows of 16385: one CTA each 10.8 us, two 14.0, four 13.6 (the cluster's
+// barriers cost more than the shorter passes save); one row of 131072: eight CTAs 26.5 us, four 40.7.
+constexpr int kLeastShare = 16384;
 constexpr int kRing = 8;  // groups that a thread has on their way when it reads a row again
-constexpr int kSearches = 16;  // lists of one row: three searches, each with up to three further cuts
+constexpr int kSearches = 24;  // lists of one row: three searches with up to four further cuts each, and three more
 constexpr int64_t kMaxVocab = int64_t(1) << 17;
 
 struct SampleArgs {
@@ -120,6 +138,19 @@ __device__ __forceinline__ u64 weight_of(float v, double top, double scale, cons
     return static_cast<u64>(__double_as_longlong(w)) & ((1ull << 52) - 1);
 }
 
+// A slice of the histogram: what lies before it, and with it.
+struct Slice {
+    int bin;
+    u64 before, upto;
+};
+
+// A row's settings, with the values out of range replaced.
+struct Settings {
+    int64_t top_k;
+    float temperature, top_p, min_p, uniform;
+    int bad;
+};
+
 // A token found: its place in the order, what lies before it, and what it has itself (weight, or 1).
 struct Found {
     u64 order, before, own;
@@ -133,8 +164,9 @@ struct Shared {
     Found found;
     u64 target;
     int place;                        // of this CTA's first token in the list
-    u64 before, upto;                 // the slice that the target falls into: what lies before it, and with it
-    int bin;
+    Slice slice, other;               // the one that the target falls into; the draw's, where it is known with top-p's
+    int joint;                        // it is
+    Settings set;
     int cursor[kSearches];            // first CTA: tokens of each list
     uint32_t most[kMaxCluster], least[kMaxCluster], ties[kMaxCluster];  // of every CTA, in every CTA
     int nan[kMaxCluster];
@@ -159,24 +191,21 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) {
     return __bfloat162float(v);
 }
 
+// 16-byte groups whose loads a thread has on their way when it reads a row that is held: the whole of a 16384-token
+// vocabulary and of the few tokens that commonly come on top of a power of two.
+template <typename T>
+constexpr int kAheadOf = sizeof(T) == 4 ? 9 : 5;
+
 template <typename T, bool CLUSTER, bool HELD>
 class Row {
    public:
-    __device__ Row(const SampleArgs &args, Shared &shared, unsigned char *dynamic) : a(args), sh(shared) {
-        lo = reinterpret_cast<uint32_t *>(dynamic);
-        hi = lo + kBins;
-        list = reinterpret_cast<u64 *>(hi + kBins);
-        spare = list + kList;
-        buf = reinterpret_cast<float *>(spare + kList);
-        ring = reinterpret_cast<uint4 *>(buf);
-        penalised = (HELD ? lo : reinterpret_cast<uint32_t *>(buf + a.slots)) + 1;
-        ignored = penalised + a.words;
+    __device__ Row(const SampleArgs &args, Shared &shared) : a(args), sh(shared) {
         tid = threadIdx.x;
         rank = CLUSTER ? static_cast<int>(cg::this_cluster().block_rank()) : 0;
         ctas = CLUSTER ? static_cast<int>(cg::this_cluster().num_blocks()) : 1;
     }
 
-    __device__ void run(int64_t row_index) {
+    __device__ __forceinline__ void run(int64_t row_index) {
         row = row_index;
         if (tid < kSearches) sh.cursor[tid] = 0;
         if (tid < kSteps) sh.powers[tid] = kStepPowers.v[tid];
@@ -185,21 +214,40 @@ class Row {
         load();
         share_extremes();
         settings();
-        if (top == -INFINITY)
-            finish(-1, 0, 1);
-        else
+        if (top == -INFINITY) {
+            if (leader() && tid == 0) {
+                a.out[row] = 0;
+                if (a.logprob) a.logprob[row] = -INFINITY;
+                flag(LEVO_SAMPLE_EMPTY);
+            }
+        } else {
             sample();
+        }
         sync_all();  // nobody leaves while another reads its shared memory
     }
 
    private:
     const SampleArgs &a;
     Shared &sh;
-    uint32_t *lo, *hi;  // histogram, then its running sums (first CTA): 64 bits in two words
-    u64 *list, *spare;
-    float *buf;                     // HELD: this CTA's logits, as the order sees them
-    uint4 *ring;                    // else: groups on their way
-    uint32_t *penalised, *ignored;  // a bit a logit, and a word to spare at both ends (HELD: in the histogram's place)
+    // The dynamic shared memory, at offsets that the compiler knows (pointers to it would hold registers).
+    static __device__ __forceinline__ unsigned char *dynamic(size_t offset) {
+        extern __shared__ __align__(16) unsigned char memory[];
+        return memory + offset;
+    }
+    // Histogram, then its running sums (first CTA): 64 bits in two words.
+    static __device__ __forceinline__ uint32_t *lo() { return reinterpret_cast<uint32_t *>(dynamic(0)); }
+    static __device__ __forceinline__ uint32_t *hi() { return lo() + kBins; }
+    static __device__ __forceinline__ u64 *list() { return reinterpret_cast<u64 *>(hi() + kBins); }
+    static __device__ __forceinline__ u64 *spare() { return list() + kList; }
+    // HELD: this CTA's logits, as the order sees them.  Else: groups on their way.
+    static __device__ __forceinline__ float *buf() { return reinterpret_cast<float *>(spare() + kList); }
+    static __device__ __forceinline__ uint4 *ring() { return reinterpret_cast<uint4 *>(spare() + kList); }
+    // A bit a logit, and a word to spare at both ends (HELD: in the histogram's place).
+    __device__ __forceinline__ uint32_t *penalised() const {
+        return (HELD ? lo() : reinterpret_cast<uint32_t *>(buf() + a.slots)) + 1;
+    }
+    __device__ __forceinline__ uint32_t *ignored() const { return penalised() + a.words; }
+
     int tid, rank, ctas, searches = 0;
     int64_t row;
     const T *x;                       // this CTA's logits
@@ -210,76 +258,69 @@ class Row {
     float half_top, reach, slices;   // slices of a unit of (top - v) / 2, which has weight up to `reach`
     int bins;
     double wide_top, scale;
-    int64_t top_k;
-    float top_p, min_p, uniform;
-    float temperature;
-    bool bad, infinite;
+    bool infinite;
     bool limited = false;  // by top-k: tokens up to (limit_value, limit_index) in the order
     float limit_value;
     int limit_index;
 
-    __device__ bool leader() const { return rank == 0; }
-    __device__ void sync_all() {
+    __device__ __forceinline__ bool leader() const { return rank == 0; }
+    __device__ __forceinline__ void sync_all() {
         if (CLUSTER)
             cg::this_cluster().sync();
         else
             __syncthreads();
     }
     template <typename U>
-    __device__ U *at(U *mine, int cta) const {
+    __device__ __forceinline__ U *at(U *mine, int cta) const {
         return CLUSTER ? cg::this_cluster().map_shared_rank(mine, cta) : mine;
     }
 
     // An empty histogram of that many slices.
-    __device__ void new_bins(int n) {
+    __device__ __forceinline__ void new_bins(int n) {
         bins = n;
         slices = fminf(__fdiv_rn(static_cast<float>(n - 1), reach), FLT_MAX);
         clear();
     }
-    __device__ void clear() {
+    __device__ __forceinline__ void clear() {
         for (int i = 4 * tid; i < bins; i += 4 * kThreads) {
-            *reinterpret_cast<uint4 *>(lo + i) = make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4 *>(hi + i) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(lo() + i) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4 *>(hi() + i) = make_uint4(0, 0, 0, 0);
         }
         __syncthreads();
     }
 
     // ---- the row -------------------------------------------------------------------------------------------
     static constexpr int L = 16 / sizeof(T);  // logits of a 16-byte group
-    // Groups whose loads a thread has on their way.  The whole of a 16384-token vocabulary and of the few tokens that
-    // commonly come on top of a power of two.
-    static constexpr int kAhead = sizeof(T) == 4 ? 9 : 5;
-
-    __device__ bool ignores() const { return a.ignore && (a.streams > 0 ? row % a.streams == 0 : row == 0); }
+    __device__ __forceinline__ bool ignores() const { return a.ignore && (a.streams > 0 ? row % a.streams == 0 : row == 0); }
 
     // The L bits of a group.
-    __device__ uint32_t bits_of(const uint32_t *words, int g) const {
+    __device__ __forceinline__ uint32_t bits_of(const uint32_t *words, int g) const {
         const int e = g * L - phase;
         return __funnelshift_r(words[e >> 5], words[(e >> 5) + 1], e & 31) & ((1u << L) - 1);
     }
     static __device__ __noinline__ float penalty_of(float v, float penalty) { return __fdiv_rn(v, penalty); }
 
     // A bit for every penalised and every ignored id of this CTA's share.
-    __device__ void mark_edits() {
-        for (int i = tid - 1; i < 2 * a.words - 1; i += kThreads) penalised[i] = 0;
+    __device__ __forceinline__ void mark_edits() {
+        for (int i = tid - 1; i < 2 * a.words - 1; i += kThreads) penalised()[i] = 0;
         __syncthreads();
         if (a.recent)
             for (int64_t j = tid; j < a.recent_len; j += kThreads) {
                 const int64_t id = a.recent[row * a.recent_len + j], e = id - start;
-                if (id >= 0 && id < a.limit && e >= 0 && e < count) atomicOr(&penalised[e >> 5], 1u << (e & 31));
+                if (id >= 0 && id < a.limit && e >= 0 && e < count) atomicOr(&penalised()[e >> 5], 1u << (e & 31));
             }
         if (ignores())
             for (int64_t j = tid; j < a.n_ignore; j += kThreads) {
                 const int64_t e = a.ignore[j] - start;
-                if (e >= 0 && e < count) atomicOr(&ignored[e >> 5], 1u << (e & 31));
+                if (e >= 0 && e < count) atomicOr(&ignored()[e >> 5], 1u << (e & 31));
             }
         __syncthreads();
     }
 
-    // f(group, logits, first, end) for each of this CTA's groups, whose logits [first, end) are the CTA's (the others
-    // are -inf); `between` runs while the first loads are on their way.  The same threads take the same groups always.
+    // f(group, logits, whole) for each of this CTA's groups (of those at both ends, what is not the CTA's is -inf);
+    // `between` runs while the first loads are on their way.  The same threads take the same groups always.
     template <typename B, typename F>
-    __device__ void read_groups(B between, F f) {
+    __device__ __forceinline__ void read_groups(B between, F f) {
         const int begin = phase > 0 ? 1 : 0, end = (phase + count) / L;  // whole groups
         const T *const base = x - phase;
         auto take = [&](const uint4 &raw, int g) {
@@ -287,9 +328,10 @@ class Row {
             float v[L];
 #pragma unroll
             for (int i = 0; i < L; ++i) v[i] = to_float(values[i]);
-            f(g, v);
+            f(g, v, true);
         };
         if constexpr (HELD) {
+            constexpr int kAhead = kAheadOf<T>;
             for (int g0 = begin + tid; g0 - tid < end || g0 == begin + tid; g0 += kAhead * kThreads) {
                 uint4 raw[kAhead];
 #pragma unroll
@@ -305,7 +347,7 @@ class Row {
             }
         } else {
             // a ring of kRing groups a thread in shared memory, which that thread alone fills and reads
-            uint4 *const own = ring + tid;
+            uint4 *const own = ring() + tid;
             auto start_copy = [&](int g, int slot) {
                 if (g < end) cp_async16(own + slot * kThreads, base + g * L);
                 cp_async_commit();
@@ -332,13 +374,13 @@ class Row {
                 const int e = g * L - phase + i;
                 v[i] = e >= 0 && e < count ? to_float(x[e]) : -INFINITY;
             }
-            f(g, v);
+            f(g, v, false);
         }
     }
 
     // Penalty and ignore list of a group read again.
-    __device__ void edit(float (&v)[L], int g) const {
-        const uint32_t p = bits_of(penalised, g), n = bits_of(ignored, g);
+    __device__ __forceinline__ void edit(float (&v)[L], int g) const {
+        const uint32_t p = bits_of(penalised(), g), n = bits_of(ignored(), g);
         if (p | n) {
 #pragma unroll
             for (int i = 0; i < L; ++i) {
@@ -348,48 +390,62 @@ class Row {
         }
     }
 
-    __device__ void load() {
+    __device__ __forceinline__ void load() {
         start = rank * a.chunk;
         count = static_cast<int>(min(static_cast<int64_t>(a.chunk), a.vocab - start));
         x = static_cast<const T *>(a.logits) + row * a.ld + start;
         phase = static_cast<int>(reinterpret_cast<uintptr_t>(x) / sizeof(T)) & (L - 1);
         groups = (phase + count + L - 1) / L;
         edits = a.recent || ignores();
-        float most = -INFINITY, least = INFINITY;
+        // Extremes: two instructions a logit that give NaN and -inf away where there is one, and then a second, careful
+        // look at the thread's logits.
+        float most = -INFINITY, least = INFINITY, quick_most = -INFINITY, quick_least = INFINITY;
         bool nan = false;
-        auto note = [&](float v) {  // neither extreme takes a NaN
+        auto note = [&](float v) {  // neither extreme takes a NaN, and the least no -inf
             nan |= isnan(v);
             most = fmaxf(most, v);
             least = fminf(least, v == -INFINITY ? INFINITY : v);
         };
-        read_groups([&] { if (edits) mark_edits(); }, [&](int g, float(&v)[L]) {
-            if (HELD) {
+        auto marks_of = [&](int g) { return edits ? bits_of(penalised(), g) | bits_of(ignored(), g) : 0u; };
+        read_groups([&] { if (edits) mark_edits(); }, [&](int g, float(&v)[L], bool full) {
+            if (HELD) {  // what is penalised or ignored is held as it came, and edited below
 #pragma unroll
                 for (int i = 0; i < L; i += 4)
-                    *reinterpret_cast<float4 *>(buf + g * L + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-                if (edits) {  // what is penalised or ignored is held as it came, and edited below
-                    const uint32_t marks = bits_of(penalised, g) | bits_of(ignored, g);
-                    if (marks) {
-#pragma unroll
-                        for (int i = 0; i < L; ++i)
-                            if (marks >> i & 1) v[i] = -INFINITY;
-                    }
-                }
+                    *reinterpret_cast<float4 *>(buf() + g * L + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
             } else if (edits) {
                 edit(v, g);
             }
+            const uint32_t marks = HELD ? marks_of(g) : 0;
+            if (full && marks == 0) {
 #pragma unroll
-            for (int i = 0; i < L; ++i) note(v[i]);
+                for (int i = 0; i < L; ++i) {
+                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(quick_most) : "f"(v[i]));
+                    quick_least = fminf(quick_least, v[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < L; ++i)
+                    if (!(marks >> i & 1)) note(v[i]);
+            }
         });
+        if (isnan(quick_most) || quick_least == -INFINITY) {
+            for (int g = (phase > 0 ? 1 : 0) + tid; g < (phase + count) / L; g += kThreads) {
+                const uint32_t marks = HELD ? marks_of(g) : 0;
+                for (int i = 0; i < L; ++i)
+                    if (!(marks >> i & 1)) note(HELD ? buf()[g * L + i] : raw_logit(g * L + i - phase));
+            }
+        } else {
+            most = fmaxf(most, quick_most), least = fminf(least, quick_least);
+        }
         if (HELD && edits) {
             __syncthreads();
-            float *const mine = buf + phase;
+            float *const mine = buf() + phase;
             if (a.recent)
                 for (int64_t j = tid; j < a.recent_len; j += kThreads) {
                     const int64_t id = a.recent[row * a.recent_len + j], e = id - start;
                     if (id < 0 || id >= a.limit || e < 0 || e >= count) continue;
                     const uint32_t bit = 1u << (e & 31);
-                    if ((ignored[e >> 5] & bit) || !(atomicAnd(&penalised[e >> 5], ~bit) & bit)) continue;  // once an id
+                    if ((ignored()[e >> 5] & bit) || !(atomicAnd(&penalised()[e >> 5], ~bit) & bit)) continue;  // once an id
                     mine[e] = penalty_of(mine[e], a.penalty);
                     note(mine[e]);
                 }
@@ -412,7 +468,7 @@ class Row {
     }
 
     // Largest and smallest key (and the NaN flag) of the row, from those of each CTA.
-    __device__ void share_extremes() {
+    __device__ __forceinline__ void share_extremes() {
         if (CLUSTER) {
             if (tid < ctas) {
                 *at(&sh.most[rank], tid) = sh.block_most;
@@ -430,24 +486,26 @@ class Row {
         lowest = value_of(least);
     }
 
-    // This row's settings (loaded ahead of the row).
-    __device__ void ask() {
-        temperature = a.temperature_rows ? a.temperature_rows[row] : a.temperature;
-        top_k = a.top_k_rows ? a.top_k_rows[row] : a.top_k;
-        top_p = a.top_p_rows ? a.top_p_rows[row] : a.top_p;
-        min_p = a.min_p_rows ? a.min_p_rows[row] : a.min_p;
-        uniform = a.uniforms[row];
+    // This row's settings, by one thread ahead of the row.
+    __device__ __forceinline__ void ask() {
+        if (tid != kThreads - 1) return;
+        Settings set{a.top_k_rows ? a.top_k_rows[row] : a.top_k,
+                     a.temperature_rows ? a.temperature_rows[row] : a.temperature,
+                     a.top_p_rows ? a.top_p_rows[row] : a.top_p, a.min_p_rows ? a.min_p_rows[row] : a.min_p,
+                     a.uniforms[row], 0};
+        float &t = set.temperature, &p = set.top_p, &m = set.min_p, &u = set.uniform;
+        if (!(t >= 0.0f) || isinf(t)) set.bad = 1, t = 0.0f;
+        if (set.top_k < 0) set.bad = 1, set.top_k = 0;
+        if (set.top_k == 0 || set.top_k > a.vocab) set.top_k = a.vocab;
+        if (!(p >= 0.0f && p <= 1.0f)) set.bad = 1, p = p < 0.0f ? 0.0f : 1.0f;
+        if (!(m >= 0.0f && m <= 1.0f)) set.bad = 1, m = m > 1.0f ? 1.0f : 0.0f;
+        if (!(u >= 0.0f && u < 1.0f)) set.bad = 1, u = u >= 1.0f ? 1.0f : 0.0f;
+        if (t == 0.0f) set.top_k = 1;
+        sh.set = set;
     }
 
-    __device__ void settings() {
-        bad = false;
-        if (!(temperature >= 0.0f) || isinf(temperature)) bad = true, temperature = 0.0f;
-        if (top_k < 0) bad = true, top_k = 0;
-        if (top_k == 0 || top_k > a.vocab) top_k = a.vocab;
-        if (!(top_p >= 0.0f && top_p <= 1.0f)) bad = true, top_p = top_p < 0.0f ? 0.0f : 1.0f;
-        if (!(min_p >= 0.0f && min_p <= 1.0f)) bad = true, min_p = min_p > 1.0f ? 1.0f : 0.0f;
-        if (!(uniform >= 0.0f && uniform < 1.0f)) bad = true, uniform = uniform >= 1.0f ? 1.0f : 0.0f;
-        if (temperature == 0.0f) top_k = 1;
+    __device__ __forceinline__ void settings() {
+        const float temperature = sh.set.temperature;
         scale = temperature > 0.0f ? kSteps * 1.4426950408889634074 / static_cast<double>(temperature) : 0.0;
         infinite = top == INFINITY;  // +inf alone has weight: as 0 among -inf
         if (infinite) {
@@ -463,12 +521,12 @@ class Row {
 
     // Slice of a logit: never smaller for a smaller logit; `bins` and above where there is no weight (-inf among it)
     // and for NaN.  The sum with 2^23 leaves the nearest integer in the low bits.
-    __device__ uint32_t bin_of(float v) const {
+    __device__ __forceinline__ uint32_t bin_of(float v) const {
         const float d = __fmaf_rn(-0.5f, v, half_top);
         return __float_as_uint(__fmaf_rn(d, slices, 8388608.0f)) - 0x4b000000u;
     }
     // A value below every logit of the slices up to `bin`: the lower edge, moved until it lies outside them.
-    __device__ float below(uint32_t bin) const {
+    __device__ __forceinline__ float below(uint32_t bin) const {
         const float width = __fdiv_rn(2.0f, slices);
         for (float past = 1.0f; past < 100.0f; past *= 4.0f) {
             const float v = __fmaf_rn(-(static_cast<float>(bin) + past), width, top);
@@ -478,7 +536,7 @@ class Row {
         return bin_of(next) > bin ? next : -INFINITY;
     }
     // A value that no logit of the slices from `bin` on lies above.
-    __device__ float above(uint32_t bin) const {
+    __device__ __forceinline__ float above(uint32_t bin) const {
         const float width = __fdiv_rn(2.0f, slices);
         for (uint32_t past = 1; past < min(bin, 100u); past *= 4) {
             const float v = __fmaf_rn(-static_cast<float>(bin - past), width, top);
@@ -486,14 +544,14 @@ class Row {
         }
         return INFINITY;
     }
-    __device__ bool within(float v, int index) const {
+    __device__ __forceinline__ bool within(float v, int index) const {
         return !limited || v > limit_value || (v == limit_value && index <= limit_index);
     }
-    __device__ u64 weight(float v) const { return weight_of(v, wide_top, scale, sh.powers); }
+    __device__ __forceinline__ u64 weight(float v) const { return weight_of(v, wide_top, scale, sh.powers); }
 
     // f(logits, index of the first) for this CTA's tokens by fours.
     template <typename F>
-    __device__ void for_fours(F f) {
+    __device__ __forceinline__ void for_fours(F f) {
         auto four = [&](float(&v)[4], int first) {
             if (infinite) {
 #pragma unroll
@@ -504,12 +562,12 @@ class Row {
         if constexpr (HELD) {
             const int quads = groups * L / 4;
             for (int g = tid; g < quads; g += kThreads) {
-                const float4 q = reinterpret_cast<const float4 *>(buf)[g];
+                const float4 q = reinterpret_cast<const float4 *>(buf())[g];
                 float v[4] = {q.x, q.y, q.z, q.w};
                 four(v, start + 4 * g - phase);
             }
         } else {
-            read_groups([] {}, [&](int g, float(&group)[L]) {
+            read_groups([] {}, [&](int g, float(&group)[L], bool) {
                 if (edits) edit(group, g);
 #pragma unroll
                 for (int i = 0; i < L; i += 4) {
@@ -522,7 +580,7 @@ class Row {
     // f(logits, slices) for this CTA's tokens by fours; a token without weight, or beyond the limit of top-k, has a
     // slice of `bins` or above.
     template <typename F>
-    __device__ void for_slices(F f) {
+    __device__ __forceinline__ void for_slices(F f) {
         for_fours([&](const float(&v)[4], int first) {
             uint32_t bin[4];
 #pragma unroll
@@ -537,37 +595,27 @@ class Row {
     }
 
     // ---- histograms ----------------------------------------------------------------------------------------
-    __device__ void add(uint32_t bin, u64 w) {
-#ifdef ADD64
-        atomicAdd(reinterpret_cast<u64 *>(lo) + bin, w);
-        return;
-#endif
+    __device__ __forceinline__ void add(uint32_t bin, u64 w) {
         const uint32_t low = static_cast<uint32_t>(w);
-        const uint32_t old = atomicAdd(&lo[bin], low);
+        const uint32_t old = atomicAdd(&lo()[bin], low);
         const uint32_t high = static_cast<uint32_t>(w >> 32) + (old + low < old);
-        if (high) atomicAdd(&hi[bin], high);
+        if (high) atomicAdd(&hi()[bin], high);
     }
 
-    __device__ void add4(const uint32_t (&bin)[4], const u64 (&w)[4]) {
-#ifdef ADD64
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (bin[i] < bins) atomicAdd(reinterpret_cast<u64 *>(lo) + bin[i], w[i]);
-#else
+    __device__ __forceinline__ void add4(const uint32_t (&bin)[4], const u64 (&w)[4]) {
         uint32_t old[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (bin[i] < bins) old[i] = atomicAdd(&lo[bin[i]], static_cast<uint32_t>(w[i]));
+            if (bin[i] < bins) old[i] = atomicAdd(&lo()[bin[i]], static_cast<uint32_t>(w[i]));
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t high = static_cast<uint32_t>(w[i] >> 32) + (old[i] + static_cast<uint32_t>(w[i]) < old[i]);
-            if (bin[i] < bins && high) atomicAdd(&hi[bin[i]], high);
+            if (bin[i] < bins && high) atomicAdd(&hi()[bin[i]], high);
         }
-#endif
     }
 
     // Running sums of the cluster's histogram, in the first CTA: a slice's words = what lies before it.
-    __device__ void running_sums() {
+    __device__ __forceinline__ void running_sums() {
         sync_all();
         if (CLUSTER) {
             constexpr int kMost = kBins / 2 / kThreads;
@@ -581,7 +629,7 @@ class Row {
 #pragma unroll
                     for (int c = 0; c < kMaxCluster; ++c) {
                         const int from = min(c, ctas - 1);  // every load unconditional: all are on their way at once
-                        const u64 part = (static_cast<u64>(*at(&hi[bin], from)) << 32) + *at(&lo[bin], from);
+                        const u64 part = (static_cast<u64>(*at(&hi()[bin], from)) << 32) + *at(&lo()[bin], from);
                         sum[i] += c < ctas ? part : 0;
                     }
                 }
@@ -591,8 +639,8 @@ class Row {
             for (int i = 0; i < kMost; ++i) {
                 const int bin = rank * share + i * kThreads + tid;
                 if (i * kThreads + tid < share) {
-                    *at(&lo[bin], 0) = static_cast<uint32_t>(sum[i]);
-                    *at(&hi[bin], 0) = static_cast<uint32_t>(sum[i] >> 32);
+                    *at(&lo()[bin], 0) = static_cast<uint32_t>(sum[i]);
+                    *at(&hi()[bin], 0) = static_cast<uint32_t>(sum[i] >> 32);
                 }
             }
             sync_all();
@@ -606,22 +654,22 @@ class Row {
 
     // A thread's N neighbouring sums.
     template <int N>
-    __device__ void sums_of(u64 (&sum)[N]) const {
+    __device__ __forceinline__ void sums_of(u64 (&sum)[N]) const {
         if constexpr (N % 4 == 0) {
 #pragma unroll
             for (int i = 0; i < N; i += 4) {
-                const uint4 l = *reinterpret_cast<const uint4 *>(lo + tid * N + i);
-                const uint4 h = *reinterpret_cast<const uint4 *>(hi + tid * N + i);
+                const uint4 l = *reinterpret_cast<const uint4 *>(lo() + tid * N + i);
+                const uint4 h = *reinterpret_cast<const uint4 *>(hi() + tid * N + i);
                 sum[i] = (static_cast<u64>(h.x) << 32) | l.x, sum[i + 1] = (static_cast<u64>(h.y) << 32) | l.y;
                 sum[i + 2] = (static_cast<u64>(h.z) << 32) | l.z, sum[i + 3] = (static_cast<u64>(h.w) << 32) | l.w;
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) sum[i] = (static_cast<u64>(hi[tid * N + i]) << 32) | lo[tid * N + i];
+            for (int i = 0; i < N; ++i) sum[i] = (static_cast<u64>(hi()[tid * N + i]) << 32) | lo()[tid * N + i];
         }
     }
     template <int N>
-    __device__ void add_up() {
+    __device__ __forceinline__ void add_up() {
         u64 own[N], sum = 0, all;
         sums_of(own);
 #pragma unroll
@@ -637,95 +685,175 @@ class Row {
         if constexpr (N % 4 == 0) {
 #pragma unroll
             for (int i = 0; i < N; i += 4) {
-                *reinterpret_cast<uint4 *>(lo + tid * N + i) = make_uint4(l[i], l[i + 1], l[i + 2], l[i + 3]);
-                *reinterpret_cast<uint4 *>(hi + tid * N + i) = make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+                *reinterpret_cast<uint4 *>(lo() + tid * N + i) = make_uint4(l[i], l[i + 1], l[i + 2], l[i + 3]);
+                *reinterpret_cast<uint4 *>(hi() + tid * N + i) = make_uint4(h[i], h[i + 1], h[i + 2], h[i + 3]);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) lo[tid * N + i] = l[i], hi[tid * N + i] = h[i];
+            for (int i = 0; i < N; ++i) lo()[tid * N + i] = l[i], hi()[tid * N + i] = h[i];
         }
         if (tid == 0) sh.total = all;
         __syncthreads();
     }
 
-    // The slice that `target` (below the total; the first CTA's) falls into, told to every CTA.
+    // First CTA: the slice that `target` (below the total) falls into.
     template <int N>
-    __device__ void find(u64 target) {
+    __device__ __forceinline__ void find_in(u64 target, Slice &to) {
         u64 sum[N];
         sums_of(sum);
-        const u64 next = tid + 1 < kThreads ? (static_cast<u64>(hi[(tid + 1) * N]) << 32) | lo[(tid + 1) * N] : sh.total;
-        if (sum[0] > target || target >= next) return;
-        int bin = tid * N;
-        u64 before = sum[0], upto = next;
+        const u64 next = tid + 1 < kThreads ? (static_cast<u64>(hi()[(tid + 1) * N]) << 32) | lo()[(tid + 1) * N] : sh.total;
+        if (sum[0] <= target && target < next) {
+            to = {tid * N, sum[0], next};
 #pragma unroll
-        for (int i = 1; i < N; ++i) {
-            if (sum[i] <= target)
-                bin = tid * N + i, before = sum[i];
-            else
-                upto = min(upto, sum[i]);
+            for (int i = 1; i < N; ++i) {
+                if (sum[i] <= target)
+                    to.bin = tid * N + i, to.before = sum[i];
+                else
+                    to.upto = min(to.upto, sum[i]);
+            }
         }
-        for (int c = 0; c < ctas; ++c) {
-            Shared &to = *at(&sh, c);
-            to.bin = bin;
-            to.before = before;
-            to.upto = upto;
-            to.target = target;
-        }
+        __syncthreads();
     }
-    __device__ void locate(u64 target) {
-        if (leader()) {
-            if (bins == kBins)
-                find<kBins / kThreads>(target);
-            else
-                find<kCountBins / kThreads>(target);
+    __device__ __forceinline__ void find(u64 target, Slice &to) {
+        if (bins == kBins)
+            find_in<kBins / kThreads>(target, to);
+        else
+            find_in<kCountBins / kThreads>(target, to);
+    }
+    // The first CTA's finds, told to the others.
+    __device__ __forceinline__ void tell(u64 target) {
+        if (leader() && tid < ctas) {
+            Shared &to = *at(&sh, tid);
+            to.target = target;
+            if (tid > 0) to.slice = sh.slice, to.other = sh.other, to.joint = sh.joint;
         }
         sync_all();
+    }
+    __device__ __forceinline__ void locate(u64 target) {
+        if (leader()) find(target, sh.slice);
+        tell(target);
+    }
+    // After top-p's slice is found: the draw's slice, where it is the same whatever token of top-p's slice is the last.
+    __device__ __forceinline__ void foresee() {
+        if (!leader()) return;
+        const u64 least = drawn(passed(sh.slice.before + 1)), most = drawn(passed(sh.slice.upto));
+        find(least, sh.other);
+        if (tid == 0) sh.joint = most < sh.other.upto;
+        __syncthreads();
+    }
+
+    // Where the logits of slices [from, to] lie, and a little more: |v - middle| <= reach.  One subtraction a logit and
+    // a minimum over four leave few quads to look at.
+    struct Zone {
+        float middle, reach;
+    };
+    __device__ __forceinline__ Zone zone(uint32_t from, uint32_t to) const {
+        const float floor = below(to), ceiling = fminf(above(from), top);
+        const float middle = 0.5f * floor + 0.5f * ceiling;
+        if (isinf(floor)) return {0.0f, INFINITY};
+        return {middle, fmaf(fabsf(middle), 1e-6f, 0.51f * ceiling - 0.51f * floor) + FLT_MIN};
+    }
+    static __device__ __forceinline__ bool near(const float (&v)[4], const Zone &z) {
+        const float d = fminf(fminf(fabsf(v[0] - z.middle), fabsf(v[1] - z.middle)),
+                              fminf(fabsf(v[2] - z.middle), fabsf(v[3] - z.middle)));
+        return d <= z.reach;
     }
 
     // Collects the tokens whose slice lies in [from, to] and whose key in [low, high] in the first CTA's list; returns
     // how many there are (kList are held).
-    __device__ int collect(uint32_t from, uint32_t to, uint32_t low = 0, uint32_t high = 0xffffffffu) {
+    __device__ __forceinline__ int collect(uint32_t from, uint32_t to, uint32_t low = 0, uint32_t high = 0xffffffffu) {
+        uint32_t quads = 0;
+        if constexpr (HELD) {
+            const Zone z = zone(from, to);
+            uint32_t bit = 1;
+            for_fours([&](const float(&v)[4], int) {
+                quads |= near(v, z) ? bit : 0;
+                bit <<= 1;
+            });
+        }
+        put(list(), from, to, low, high, quads);
+        sync_all();
+        return *at(&sh.cursor[searches++], 0);
+    }
+    // Both located slices, the second in the histogram's place.
+    __device__ __forceinline__ void collect_both(int &n, int &other_n) {
+        const uint32_t p = sh.slice.bin, d = sh.other.bin;
+        uint32_t quads = 0, other_quads = 0;
+        if constexpr (HELD) {
+            const Zone z = zone(p, p), other = zone(d, d);
+            uint32_t bit = 1;
+            for_fours([&](const float(&v)[4], int) {
+                quads |= near(v, z) ? bit : 0;
+                other_quads |= near(v, other) ? bit : 0;
+                bit <<= 1;
+            });
+        }
+        if constexpr (HELD) {
+#pragma unroll 1
+            for (int i = 0; i < 2; ++i, ++searches)
+                put(i ? reinterpret_cast<u64 *>(lo()) : list(), i ? d : p, i ? d : p, 0, 0xffffffffu,
+                    i ? other_quads : quads);
+        } else {
+            const Zone z = zone(p, p), other = zone(d, d);
+            for_fours([&](const float(&v)[4], int first) {
+                if (!near(v, z) && !near(v, other)) return;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t bin = bin_of(v[i]);
+                    if ((bin != p && bin != d) || !within(v[i], first + i)) continue;
+                    for (int which = 0; which < 2; ++which) {
+                        if (bin != (which ? d : p)) continue;
+                        const int place = atomicAdd(at(&sh.cursor[searches + which], 0), 1);
+                        if (place < kList)
+                            at(which ? reinterpret_cast<u64 *>(lo()) : list(), 0)[place] = order_of(v[i], first + i);
+                    }
+                }
+            });
+            searches += 2;
+        }
+        sync_all();
+        n = *at(&sh.cursor[searches - 2], 0);
+        other_n = *at(&sh.cursor[searches - 1], 0);
+    }
+
+    // This CTA's tokens of slices [from, to] and keys [low, high] to the first CTA's list.  HELD: `quads` has a bit for
+    // each of the thread's fours that can hold one; the threads' places come by a running sum.
+    __device__ __forceinline__ void put(u64 *into, uint32_t from, uint32_t to, uint32_t low, uint32_t high, uint32_t quads) {
         int *const cursor = at(&sh.cursor[searches], 0);
-        u64 *const into = at(list, 0);
+        into = at(into, 0);
         auto member = [&](float v, int index) {
             const uint32_t key = key_of(v);
             return bin_of(v) - from <= to - from && key >= low && key <= high && within(v, index);
         };
-        // all but a few fail the two comparisons
-        const float floor = below(to), ceiling = above(from);
         if constexpr (HELD) {
-            // a bit a logit of the thread's, then the threads' places by a running sum
-            static_assert(112 * 1024 / sizeof(float) <= 64 * kThreads, "a thread's logits have a bit each");
-            u64 near = 0, mine = 0;
-            int shift = 0;
-            for_fours([&](const float(&v)[4], int) {
-                uint32_t bits = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) bits |= (v[i] > floor && v[i] <= ceiling ? 1u : 0u) << i;
-                near |= static_cast<u64>(bits) << shift;
-                shift += 4;
-            });
-            auto place_of = [&](int bit) { return 4 * (tid + (bit >> 2) * kThreads) + (bit & 3); };
-            auto held = [&](int e) { return infinite ? 0.0f : buf[e]; };
-            for (; near != 0; near &= near - 1) {
-                const int bit = __ffsll(near) - 1, e = place_of(bit);
-                if (member(held(e), start + e - phase)) mine |= 1ull << bit;
+            static_assert(112 * 1024 / sizeof(float) <= 16 * 4 * kThreads, "a thread's fours have a bit each, their logits 64");
+            u64 mine = 0;
+            auto held = [&](int e) {
+                const float v = buf()[e];
+                return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
+            };
+            for (; quads != 0; quads &= quads - 1) {
+                const int quad = __ffs(quads) - 1, e = 4 * (tid + quad * kThreads);
+                for (int i = 0; i < 4; ++i)
+                    if (member(held(e + i), start + e + i - phase)) mine |= 1ull << (4 * quad + i);
             }
             u64 all;
             int place = static_cast<int>(sum_before(static_cast<u64>(__popcll(mine)), all));
-            if (tid == 0) sh.place = atomicAdd(cursor, static_cast<int>(all));
-            __syncthreads();
-            place += sh.place;
+            if (CLUSTER) {
+                if (tid == 0) sh.place = atomicAdd(cursor, static_cast<int>(all));
+                __syncthreads();
+                place += sh.place;
+            } else if (tid == 0) {
+                *cursor = static_cast<int>(all);
+            }
             for (; mine != 0 && place < kList; mine &= mine - 1, ++place) {
-                const int e = place_of(__ffsll(mine) - 1);
+                const int bit = __ffsll(mine) - 1, e = 4 * (tid + (bit >> 2) * kThreads) + (bit & 3);
                 into[place] = order_of(held(e), start + e - phase);
             }
         } else {
+            const Zone z = zone(from, to);
             for_fours([&](const float(&v)[4], int first) {
-                bool any = false;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) any |= v[i] > floor && v[i] <= ceiling;
-                if (!any) return;
+                if (!near(v, z)) return;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     if (!member(v[i], first + i)) continue;
@@ -734,15 +862,12 @@ class Row {
                 }
             });
         }
-        sync_all();
-        ++searches;
-        return *cursor;
     }
 
     // First CTA: the n listed tokens in order, one a thread (all ones behind them).  Up to a warp's: a bitonic network.
     // More: slices of the list's own range, each token's place is the slice's start and its rank in the slice (few
     // tokens, unless they are equal).  The histogram is not touched.
-    __device__ u64 sorted(int n) {
+    __device__ __forceinline__ u64 sorted(u64 *list, int n) {
         u64 mine = tid < n ? list[tid] : ~0ull;
         if (n <= 32) {
             if (tid < 32) {
@@ -778,13 +903,13 @@ class Row {
         sh.places[tid] = before;
         sh.ends[tid] = before;
         __syncthreads();
-        if (tid < n) spare[atomicAdd(&sh.ends[part], 1)] = mine;
+        if (tid < n) spare()[atomicAdd(&sh.ends[part], 1)] = mine;
         __syncthreads();
         int place = 0;
         if (tid < n) {
             const int from = sh.places[part], to = sh.ends[part];
             place = from;
-            for (int i = from; i < to; ++i) place += spare[i] < mine;
+            for (int i = from; i < to; ++i) place += spare()[i] < mine;
             list[place] = mine;
         }
         __syncthreads();
@@ -792,7 +917,7 @@ class Row {
     }
 
     // Running sum over the CTA's threads (what lies before this one); `all`: the whole.
-    __device__ u64 sum_before(u64 own, u64 &all) {
+    __device__ __forceinline__ u64 sum_before(u64 own, u64 &all) {
         u64 upto = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -812,32 +937,45 @@ class Row {
         return before;
     }
 
-    static __device__ float value_in(u64 order) { return value_of(~static_cast<uint32_t>(order >> 32)); }
-    static __device__ int index_in(u64 order) { return static_cast<int>(static_cast<uint32_t>(order)); }
+    static __device__ __forceinline__ float value_in(u64 order) { return value_of(~static_cast<uint32_t>(order >> 32)); }
+    static __device__ __forceinline__ int index_in(u64 order) { return static_cast<int>(static_cast<uint32_t>(order)); }
 
     // First CTA: which of the n listed tokens the target falls into.
-    __device__ void rank_list(int n, u64 before, u64 target, bool by_weight) {
-        const u64 mine = sorted(n);
-        const u64 own = tid >= n ? 0 : by_weight ? weight(value_in(mine)) : 1;
-        u64 all;
-        const u64 sum = before + sum_before(own, all);
-        if (sum <= target && target < sum + own) sh.found = {mine, sum, own};
+    __device__ __forceinline__ void rank_list(u64 *list, int n, u64 before, u64 target, bool by_weight) {
+        if (n <= 32) {  // a warp a token, or two: what lies before it is added up over the lanes
+            const int lane = tid & 31;
+            const u64 theirs = lane < n ? list[lane] : ~0ull;
+            const u64 own = lane >= n ? 0 : by_weight ? weight(value_in(theirs)) : 1;
+            for (int i = tid >> 5; i < n; i += kWarps) {
+                const u64 mine = __shfl_sync(0xffffffffu, theirs, i);
+                u64 sum = theirs < mine ? own : 0;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane == i && before + sum <= target && target < before + sum + own) sh.found = {mine, before + sum, own};
+            }
+        } else {
+            const u64 mine = sorted(list, n);
+            const u64 own = tid >= n ? 0 : by_weight ? weight(value_in(mine)) : 1;
+            u64 all;
+            const u64 sum = before + sum_before(own, all);
+            if (sum <= target && target < sum + own) sh.found = {mine, sum, own};
+        }
         __syncthreads();
     }
 
     // The token of the located slice that the target falls into: in the first CTA's sh.found.  A slice with too many
     // tokens costs the histogram (returns false then).
-    __device__ bool search_slice(bool by_weight) {
-        const uint32_t slice = sh.bin;
-        u64 before = sh.before;
+    __device__ __forceinline__ bool search_slice(bool by_weight) {
+        const uint32_t slice = sh.slice.bin;
+        u64 before = sh.slice.before;
         const u64 target = sh.target;
-        int n = collect(slice, slice);
-        if (n <= kList) {
-            if (leader()) rank_list(n, before, target, by_weight);
-            return true;
-        }
         uint32_t low_key = 0, high_key = 0xffffffffu;
-        for (;;) {
+        for (bool whole = true;; whole = false) {
+            const int n = collect(slice, slice, low_key, high_key);
+            if (n <= kList) {
+                if (leader()) rank_list(list(), n, before, target, by_weight);
+                return whole;
+            }
             auto member = [&](float v, uint32_t bin) {
                 const uint32_t key = key_of(v);
                 return bin == slice && key >= low_key && key <= high_key;
@@ -894,30 +1032,29 @@ class Row {
             });
             running_sums();
             locate(target - before);
-            before += sh.before;
-            high_key = most - (static_cast<uint32_t>(sh.bin) << shift);
+            before += sh.slice.before;
+            high_key = most - (static_cast<uint32_t>(sh.slice.bin) << shift);
             low_key = max(least, high_key - ((1u << shift) - 1));
-            n = collect(slice, slice, low_key, high_key);
-            if (n <= kList) {
-                if (leader()) rank_list(n, before, target, by_weight);
-                return false;
-            }
         }
     }
 
-    // One of this CTA's logits as the order sees it.
-    __device__ float logit(int i) const {
-        float v = HELD ? buf[phase + i] : to_float(x[i]);
+    // One of this CTA's logits, penalised and ignored as it may be; and as the order sees it.
+    __device__ __forceinline__ float raw_logit(int i) const {
+        float v = HELD ? buf()[phase + i] : to_float(x[i]);
         if (!HELD && edits) {
             const uint32_t bit = 1u << (i & 31);
-            if (penalised[i >> 5] & bit) v = penalty_of(v, a.penalty);
-            if (ignored[i >> 5] & bit) v = -INFINITY;
+            if (penalised()[i >> 5] & bit) v = penalty_of(v, a.penalty);
+            if (ignored()[i >> 5] & bit) v = -INFINITY;
         }
+        return v;
+    }
+    __device__ __forceinline__ float logit(int i) const {
+        const float v = raw_logit(i);
         return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
     }
 
     // Index of this CTA's n-th (from 0) token with that logit: in the thread that holds it, -1 in the others.
-    __device__ int nth(float value, uint32_t n) {
+    __device__ __forceinline__ int nth(float value, uint32_t n) {
         uint32_t before = 0;
         int found = -1;
         for (int i0 = 0; i0 < count && before <= n; i0 += kThreads) {
@@ -938,160 +1075,189 @@ class Row {
     }
 
     // ---- the filters and the draw ----------------------------------------------------------------------------
-    __device__ u64 least_weight() const {
-        return static_cast<u64>(ceil(static_cast<double>(min_p) * 17592186044416.0));  // 2^44
+    __device__ __forceinline__ u64 least_weight() const {
+        return static_cast<u64>(ceil(static_cast<double>(sh.set.min_p) * 17592186044416.0));  // 2^44
     }
 
-    // The slice that holds the k-th largest of the threads' largest logits: k tokens or more lie up to it, and few more
-    // where k is well below the number of threads.  `bins` where the threads have fewer than k.
-    __device__ int enough_for(int64_t k) {
-        const uint32_t bin = bin_of(thread_top);
-        if (bin < bins) atomicAdd(&lo[bin], 1u);
-        running_sums();
-        locate(leader() ? min(static_cast<u64>(k), sh.total) - 1 : 0);
-        return sh.target + 1 == static_cast<u64>(k) ? sh.bin : bins;
+    __device__ __forceinline__ void count_slices() {
+        for_slices([&](const float(&)[4], const uint32_t(&bin)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (bin[i] < bins) atomicAdd(&lo()[bin[i]], 1u);
+        });
     }
 
-    // The histogram of counts, or of weights (and then what min-p leaves of them, to the first CTA), and its running
-    // sums.
-    __device__ void histogram(bool of_weights) {
-        if (!of_weights) {
-            for_slices([&](const float(&)[4], const uint32_t(&bin)[4]) {
+    // The histogram of weights and its running sums; what min-p leaves of them to the first CTA.
+    __device__ __forceinline__ void weigh() {
+        const u64 least = least_weight();
+        const bool counted = sh.set.min_p > 0.0f;
+        u64 passing = 0;
+        for_slices([&](const float(&v)[4], const uint32_t(&bin)[4]) {
+            if (min(min(bin[0], bin[1]), min(bin[2], bin[3])) >= bins) return;
+            u64 w[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (bin[i] < bins) atomicAdd(&lo[bin[i]], 1u);
-            });
-        } else {
-            const u64 least = least_weight();
-            const bool counted = min_p > 0.0f;
-            u64 passing = 0;
-            for_slices([&](const float(&v)[4], const uint32_t(&bin)[4]) {
-                if (min(min(bin[0], bin[1]), min(bin[2], bin[3])) >= bins) return;
-                u64 w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = weight(bin[i] < bins ? v[i] : top);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (counted && bin[i] < bins && w[i] >= least) passing += w[i];
-                add4(bin, w);
-            });
-            if (min_p > 0.0f) {
-                u64 all;
-                sum_before(passing, all);
-                if (tid == 0) at(&sh, 0)->passing[rank] = all;
+            for (int i = 0; i < 4; ++i) {
+                w[i] = weight(bin[i] < bins ? v[i] : top);
             }
+            if (counted) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (bin[i] < bins && w[i] >= least) passing += w[i];
+            }
+            add4(bin, w);
+        });
+        if (counted) {
+            u64 all;
+            sum_before(passing, all);
+            if (tid == 0) at(&sh, 0)->passing[rank] = all;
         }
         running_sums();
     }
 
-    // Weight that is kept of `all`: up to the token that passes top-p, and no more than min-p lets pass.
-    __device__ u64 drawn(u64 kept) const {
-        const u64 place = static_cast<u64>(static_cast<double>(uniform) * static_cast<double>(kept));
+    // The weight whose token is drawn, and the one whose token is the last that top-p keeps.
+    __device__ __forceinline__ u64 drawn(u64 kept) const {
+        const u64 place = static_cast<u64>(static_cast<double>(sh.set.uniform) * static_cast<double>(kept));
         return min(place, kept - 1);
     }
-    __device__ u64 nucleus(u64 all) const {  // the weight whose token is the last that top-p keeps
-        const u64 part = static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(all)));
+    __device__ __forceinline__ u64 nucleus(u64 all) const {
+        const u64 part = static_cast<u64>(ceil(static_cast<double>(sh.set.top_p) * static_cast<double>(all)));
         return max(part, u64(1)) - 1;
+    }
+    // First CTA: what min-p leaves of a kept weight (both filters keep a prefix).
+    __device__ __forceinline__ u64 passed(u64 kept) const {
+        if (!(sh.set.min_p > 0.0f)) return kept;
+        u64 passing = 0;
+        for (int c = 0; c < ctas; ++c) passing += sh.passing[c];
+        return min(kept, passing);
     }
 
     // First CTA: all that can be drawn is in the list (n tokens and no more): filters and draw over it in order.
-    __device__ void sample_list(int n) {
-        const u64 mine = sorted(n);
-        const u64 own = tid < min(static_cast<int64_t>(n), top_k) ? weight(value_in(mine)) : 0;
+    __device__ __forceinline__ void sample_list(int n) {
+        const u64 mine = sorted(list(), n);
+        const u64 own = tid < min(static_cast<int64_t>(n), sh.set.top_k) ? weight(value_in(mine)) : 0;
         u64 kept, passing;
         const u64 before = sum_before(own, kept);
-        if (top_p < 1.0f) {
+        if (sh.set.top_p < 1.0f) {
             const u64 target = nucleus(kept);
             if (before <= target && target < before + own) sh.total = before + own;
             __syncthreads();
             kept = sh.total;
         }
-        if (min_p > 0.0f) {
+        if (sh.set.min_p > 0.0f) {
             sum_before(own >= least_weight() ? own : 0, passing);
             kept = min(kept, passing);
         }
         const u64 target = drawn(kept);
-        if (before <= target && target < before + own) sh.found = {mine, before, own};
-        __syncthreads();
-        finish(index_in(sh.found.order), sh.found.own, kept);
+        if (before <= target && target < before + own) finish(mine, own, kept);
     }
 
-    __device__ void sample() {
-        enum { kTopK, kTopP, kDraw } stage = top_k < a.vocab ? kTopK : top_p < 1.0f ? kTopP : kDraw;
-        bool fresh = true;  // the stage needs a histogram of its own
-        u64 kept = 0;       // first CTA: weight that is kept
-        new_bins(stage == kTopK ? kCountBins : kBins);
-        if (a.vocab <= kList) {
-            const int n = collect(0, bins - 1);
-            if (leader()) sample_list(n);
-            return;
-        }
-        if (stage == kTopK && top_k <= kList) {
-            const int slice = enough_for(top_k);
-            if (slice < bins) {
-                const int n = collect(0, slice);
-                if (n <= kList) {
-                    if (leader()) sample_list(n);
-                    return;
-                }
-            }
-            sync_all();  // the histogram has been read
+    __device__ __forceinline__ void sample() {
+        const int64_t top_k = sh.set.top_k;
+        const bool has_top_p = sh.set.top_p < 1.0f;
+        enum { kTopK, kTopP, kDraw } stage = top_k < a.vocab ? kTopK : has_top_p ? kTopP : kDraw;
+
+        // Few candidates: the first CTA has them all.  A short vocabulary; the tokens down to the k-th largest of the
+        // threads' largest; the tokens up to the k-th one's slice (or to the last slice with a token).
+#pragma unroll 1
+        for (int attempt = a.vocab <= kList ? 0 : stage != kTopK ? 3 : top_k <= kList ? 1 : 2; attempt < 3; ++attempt) {
+            if (attempt != 1) sync_all();  // the histogram before has been read
             new_bins(kCountBins);
-        }
-        for (;;) {
-            if (fresh) {
-                histogram(stage != kTopK);
-                if (stage != kTopK && kept == 0) kept = leader() ? sh.total : 0;
+            int upto = bins - 1;
+            if (attempt > 0) {
+                if (attempt == 1) {
+                    const uint32_t bin = bin_of(thread_top);
+                    if (bin < bins) atomicAdd(&lo()[bin], 1u);
+                } else {
+                    count_slices();
+                }
+                running_sums();
+                locate(leader() ? min(static_cast<u64>(top_k), sh.total) - 1 : 0);
+                upto = sh.slice.bin;
+                // the threads have fewer than k tokens of weight; the slices have too many
+                if (attempt == 1 ? sh.target + 1 < static_cast<u64>(top_k) : sh.slice.upto > kList) continue;
             }
-            if (stage == kDraw && min_p > 0.0f && leader()) {
-                u64 passing = 0;
-                for (int c = 0; c < ctas; ++c) passing += sh.passing[c];
-                kept = min(kept, passing);
-            }
-            u64 target = 0;
-            if (leader())
-                target = stage == kTopK ? min(static_cast<u64>(top_k), sh.total) - 1
-                         : stage == kTopP ? nucleus(kept)
-                                          : drawn(kept);
-            locate(target);
-            // Few tokens up to the k-th one's slice (or the last slice with a token): the first CTA has them all.
-            if (stage == kTopK && sh.upto <= kList) {
-                const int n = collect(0, sh.bin);
+            const int n = collect(0, upto);
+            if (n <= kList) {
                 if (leader()) sample_list(n);
                 return;
             }
-            bool whole = false;
-            if (stage != kTopK || sh.target + 1 == static_cast<u64>(top_k)) {
-                whole = search_slice(stage != kTopK);
-                if (stage == kTopK) {
-                    if (CLUSTER) {
-                        if (leader() && tid > 0 && tid < ctas) at(&sh, tid)->found = sh.found;
-                        sync_all();
+        }
+
+        // One search after the other, each for a target in the running sums of its histogram.
+        bool located = stage == kTopK, fresh = false, both = true;
+        u64 kept = 0;  // first CTA: weight that top-p keeps
+        if (located && sh.target + 1 < static_cast<u64>(top_k)) located = false, stage = has_top_p ? kTopP : kDraw;
+        if (!located) fresh = true;
+        for (;;) {
+            if (fresh) {
+                sync_all();  // the histogram before has been read
+                new_bins(kBins);
+                weigh();
+                if (leader() && stage == kTopP) kept = sh.total;
+                if (leader() && stage == kDraw && !has_top_p) kept = sh.total;
+            }
+            if (!located) {
+                u64 target = 0;
+                if (leader()) target = stage == kTopP ? nucleus(kept) : drawn(passed(kept));
+                const bool try_both = stage == kTopP && both;
+                if (leader()) find(target, sh.slice);
+                if (try_both) foresee();
+                tell(target);
+                if (try_both && sh.joint) {
+                    int n, other_n;
+                    collect_both(n, other_n);
+                    if (n <= kList && other_n <= kList) {
+                        if (leader()) draw_both(n, other_n);
+                        return;
                     }
-                    limited = true;
-                    limit_value = value_in(sh.found.order);
-                    limit_index = index_in(sh.found.order);
+                    both = false, fresh = true;  // one at a time then: a list has taken the histogram's place
+                    continue;
                 }
             }
+            located = false;
+            const bool whole = search_slice(stage != kTopK);
             if (stage == kDraw) break;
-            if (stage == kTopP) kept = leader() ? sh.found.before + sh.found.own : 0;
-            fresh = stage == kTopK || !whole;
-            stage = stage == kTopK && top_p < 1.0f ? kTopP : kDraw;
-            if (fresh) {
-                sync_all();  // the histograms have been read
-                new_bins(kBins);
+            if (stage == kTopK) {
+                if (CLUSTER) {
+                    if (leader() && tid > 0 && tid < ctas) at(&sh, tid)->found = sh.found;
+                    sync_all();
+                }
+                limited = true;
+                limit_value = value_in(sh.found.order);
+                limit_index = index_in(sh.found.order);
+                stage = has_top_p ? kTopP : kDraw;
+                fresh = true;
+            } else {
+                if (leader()) kept = sh.found.before + sh.found.own;
+                stage = kDraw;
+                fresh = !whole;
             }
         }
-        finish(index_in(sh.found.order), sh.found.own, kept);
+        if (leader() && tid == 0) finish(sh.found.order, sh.found.own, passed(kept));
     }
 
-    __device__ void finish(int token, u64 own, u64 kept) {
-        if (!leader() || tid != 0) return;
-        a.out[row] = max(token, 0);
+    // First CTA: top-p's token, then the draw's, of the two lists.
+    __device__ __forceinline__ void draw_both(int n, int other_n) {
+        u64 kept = 0;
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+            rank_list(i ? reinterpret_cast<u64 *>(lo()) : list(), i ? other_n : n, i ? sh.other.before : sh.slice.before,
+                      i ? drawn(kept) : sh.target, true);
+            if (i == 0) kept = passed(sh.found.before + sh.found.own);
+            __syncthreads();
+        }
+        if (tid == 0) finish(sh.found.order, sh.found.own, kept);
+    }
+
+    // One thread of the first CTA: the token and its share of what was kept.
+    __device__ __forceinline__ void finish(u64 order, u64 own, u64 kept) {
+        a.out[row] = index_in(order);
         if (a.logprob)
-            a.logprob[row] = token < 0 ? -INFINITY
-                                       : static_cast<float>(log(static_cast<double>(own) / static_cast<double>(kept)));
-        int flags = (token < 0 ? LEVO_SAMPLE_EMPTY : 0) | (bad ? LEVO_SAMPLE_PARAM : 0);
+            a.logprob[row] = static_cast<float>(log(static_cast<double>(own) / static_cast<double>(kept)));
+        flag(0);
+    }
+    __device__ __forceinline__ void flag(int flags) {
+        if (sh.set.bad) flags |= LEVO_SAMPLE_PARAM;
         for (int c = 0; c < ctas; ++c) flags |= sh.nan[c] ? LEVO_SAMPLE_NAN : 0;
         if (a.status && flags) atomicOr(a.status, flags);
     }
@@ -1099,24 +1265,22 @@ class Row {
 
 template <typename T, bool CLUSTER, bool HELD>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
-    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ Shared shared;
-    Row<T, CLUSTER, HELD> row(a, shared, dynamic);
+    Row<T, CLUSTER, HELD> row(a, shared);
     row.run(CLUSTER ? blockIdx.x / cg::this_cluster().num_blocks() : blockIdx.x);
 }
 
-#ifndef MINV
-#define MINV 4096
-#endif
 template <typename T>
 int launch_sample(SampleArgs &a, const char *what, cudaStream_t stream) {
     constexpr int L = 16 / sizeof(T);
     // As many CTAs a row as the SMs (two CTAs each) take at once, each with a share that is worth it.
     int ctas = 1;
-    while (ctas < kMaxCluster && a.rows * ctas * 2 <= 2LL * sm_count() && a.vocab / ctas >= 2 * MINV) ctas *= 2;
+    while (ctas < kMaxCluster && a.rows * ctas * 2 <= 2LL * sm_count() && a.vocab / ctas >= 2 * kLeastShare) ctas *= 2;
     a.chunk = static_cast<int>((a.vocab + ctas - 1) / ctas + 7) / 8 * 8;
     a.words = a.recent || a.ignore ? (a.chunk + 31) / 32 + 2 : 0;
-    // A share that leaves room for two CTAs an SM is held in shared memory, a longer one read again from L2.
+    // A share that leaves room for two CTAs an SM is held in shared memory (192 rows of 16385: 17.0 us; read again,
+    // 29); a longer one is read again from L2 (128 rows of 131072: two CTAs a row that read again 102 us, eight that
+    // hold their shares 153: four rounds of clusters).
     const size_t rest = 2 * kBins * sizeof(uint32_t) + 2 * kList * sizeof(u64);
     a.slots = (a.chunk + 2 * L + 3) / 4 * 4;
     const bool held = rest + a.slots * sizeof(float) + sizeof(Shared) <= 112 * 1024;
