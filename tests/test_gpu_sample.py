@@ -3,11 +3,14 @@ wrong; and the distribution that a grid of uniform numbers draws."""
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 import torch
 
+from conftest import ROOT
 from token_step_reference import DTYPES, logprob_tolerance, penalised, sample_row
 
 pytestmark = pytest.mark.gpu
@@ -22,9 +25,9 @@ def run(ops, logits, u, dev, **kw):
 
 
 def check(ops, dev, logits, u, expect_status=0, **kw):
-    """Tokens equal to the definition's and logprobs within the rounding of the weights."""
+    """Tokens equal to the definition's and logprobs within the rounding of the weights; status as expected, with
+    SAMPLE_EMPTY where the definition finds a row without a token."""
     tokens, logprobs, status = run(ops, logits, u, dev, **kw)
-    assert status == expect_status
     rows, vocab = logits.shape
     x = penalised(logits, None if kw.get("recent") is None else kw["recent"].cpu().numpy(), kw.get("penalty", 1.0),
                   kw.get("penalty_limit", 0), None if kw.get("ignore") is None else kw["ignore"].cpu().numpy(),
@@ -39,12 +42,14 @@ def check(ops, dev, logits, u, expect_status=0, **kw):
     for r, (temperature, top_k, top_p, min_p, uniform) in enumerate(settings):
         want = sample_row(x[r], uniform, temperature, top_k, top_p, min_p)
         if want is None:
+            expect_status |= ops.SAMPLE_EMPTY
             assert tokens[r] == 0 and logprobs[r] == -np.inf
             continue
         token, logprob, weight, total, near = want
         assert tokens[r] == token, f"row {r}: {tokens[r]}, not {token} ({near:.3g} from a border)"
         tol = logprob_tolerance(logprob, weight, total, vocab)
         assert abs(logprobs[r] - logprob) <= tol, f"row {r}: logprob {logprobs[r]} not {logprob} +- {tol}"
+    assert status == expect_status
     return tokens
 
 
@@ -151,6 +156,52 @@ def test_sample_clusters_of_close_logits(ops, dev):
     check(ops, dev, base, uniforms(gen, 6), top_k=9999, top_p=0.7)
     check(ops, dev, base, uniforms(gen, 6), temperature=1e-6)
     check(ops, dev, base, uniforms(gen, 6), temperature=1e6, top_p=0.3)
+
+
+# Rows x vocabulary by how a row is worked on: one CTA that holds it; one that reads it again; a cluster that holds its
+# shares; a cluster that reads them again; a single list.
+SHARES = [(7, 16385), (300, 20011), (2, 131072), (5, 50257), (40, 131071), (9, 512)]
+
+
+@pytest.mark.parametrize("rows,vocab", SHARES)
+@pytest.mark.parametrize("name", ["none", "k50", "k1500", "p999", "all", "m0.1", "zero"])
+def test_sample_hard_rows_whatever_the_split(ops, dev, rows, vocab, name):
+    """Ties, masks, infinities and edited ids in every split of the work; the edited ids lie at the shares' ends too."""
+    gen = torch.Generator(device=dev).manual_seed(vocab + rows)
+    t = list(DTYPES.values())[rows % 3]
+    x = (2 * torch.randn((rows, vocab + 3), generator=gen, device=dev)).to(t)[:, 1:vocab + 1]
+    x[0] = torch.randint(0, 5, (vocab,), generator=gen, device=dev).to(t)        # thousands of equal logits
+    x[1, ::2] = -math.inf
+    if rows > 2:
+        x[2] = 0.25
+        x[3, 5:vocab - 2] = torch.finfo(t).min
+        x[4, torch.randint(0, vocab, (3,), generator=gen, device=dev)] = math.inf
+    if rows > 6:
+        x[5] = (x[5].float() * 1e-4 + 9).to(t)
+        x[6, :-1] = -math.inf
+    edges = torch.tensor([0, 1, vocab // 2 - 1, vocab // 2, vocab - 1, vocab - 2, -1, vocab + 5], device=dev)
+    recent = torch.cat((edges.expand(rows, -1), torch.randint(-1, vocab, (rows, 600), generator=gen, device=dev)), 1)
+    top = x.float().topk(3, dim=1).indices
+    recent = torch.cat((recent, top), 1).contiguous()
+    ignore = torch.cat((edges, top[0], torch.randint(0, vocab, (700,), generator=gen, device=dev)))
+    u = uniforms(gen, rows)
+    check(ops, dev, x, u, **FILTERS[name])
+    check(ops, dev, x, u, recent=recent, penalty=1.2, penalty_limit=vocab - 1, ignore=ignore, streams=2, **FILTERS[name])
+
+
+@pytest.mark.parametrize("rows,vocab", SHARES)
+def test_sample_nan_whatever_the_split(ops, dev, rows, vocab):
+    gen = torch.Generator(device=dev).manual_seed(rows)
+    x = torch.randn((rows, vocab), generator=gen, device=dev)
+    u = uniforms(gen, rows)
+    for place in (0, vocab // 3, vocab - 1):
+        y = x.clone()
+        y[rows - 1, place] = math.nan
+        check(ops, dev, y, u, expect_status=ops.SAMPLE_NAN, top_p=0.9)
+        listed = torch.tensor([place], device=dev)
+        check(ops, dev, y, u, ignore=listed, streams=1, top_k=30)  # an ignored NaN is no NaN
+        y[rows - 1] = math.nan
+        check(ops, dev, y, u, expect_status=ops.SAMPLE_NAN | ops.SAMPLE_EMPTY, top_k=3)
 
 
 def test_sample_nan(ops, dev):
@@ -290,6 +341,24 @@ def test_sample_captured_and_replayed_beside_another_graph(ops, dev):
         torch.cuda.synchronize()
         for _, x, u, out, kw in cases:
             assert torch.equal(out, ops.sample_tokens_t(x, u, **kw))
+
+
+def test_sample_first_call_of_a_process_under_capture(dev):
+    """Kernels are loaded and opt in to their shared memory inside a capture, without a call before it."""
+    code = (
+        "import sys; sys.path.insert(0, %r); import torch, __graft_entry__ as e; ops = e.load_package().ops\n"
+        "x, u = torch.randn(3, 16385, device='cuda'), torch.rand(3, device='cuda')\n"
+        "q = torch.randn(2, 700, 12, 128, device='cuda', dtype=torch.float16)\n"
+        "out, turned = torch.zeros(3, dtype=torch.int64, device='cuda'), torch.empty_like(q)\n"
+        "theta = ops.rope_theta(128, device='cuda')\n"
+        "g = torch.cuda.CUDAGraph()\n"
+        "with torch.cuda.graph(g):\n"
+        "    ops.sample_tokens_t(x, u, top_p=0.9, out=out); ops.rope_qk_t(q, None, theta, q_out=turned)\n"
+        "g.replay(); torch.cuda.synchronize()\n"
+        "assert torch.equal(out, ops.sample_tokens_t(x, u, top_p=0.9))\n"
+        "assert torch.equal(turned, ops.rope_qk_t(q, None, theta)[0]); print('captured')\n" % str(ROOT))
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "captured" in out.stdout, out.stderr[-2000:]
 
 
 def test_sample_is_the_same_every_time_and_on_other_streams(ops, dev):

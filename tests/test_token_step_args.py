@@ -64,6 +64,18 @@ def test_rope_refuses_misaligned_pointers_and_other_strides_in_place(ops, buf):
     assert lib.levo_rope_qk(ctypes.byref(r), None) == ops.EINVAL  # a broadcast output
 
 
+def test_rope_limits(ops, buf):
+    p = ctypes.addressof(buf)
+    lib = ops.lib()
+    wide = dict(head_dim=8194, rotary_dim=8, q__heads=1, k__heads=0, batch=1, tokens=1)
+    assert lib.levo_rope_qk(ctypes.byref(rope_args(ops, p, **wide)), None) == ops.EUNSUPPORTED
+    assert "8192" in ops.last_error()
+    far = dict(batch=1 << 16, tokens=1 << 16, k__heads=0, q__heads=1, q__in_stride_batch=0, q__in_stride_token=0,
+               q__out_stride_batch=1 << 20, q__out_stride_token=16)
+    assert lib.levo_rope_qk(ctypes.byref(rope_args(ops, p, **far)), None) == ops.EUNSUPPORTED
+    assert "too many tokens" in ops.last_error()
+
+
 def test_rope_zero_sizes_are_noops(ops, buf):
     p = ctypes.addressof(buf)
     lib = ops.lib()
