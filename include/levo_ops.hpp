@@ -103,6 +103,29 @@ inline void add_layer_norm_f32(const float *x, const float *residual, const floa
                           detail::kFlowEstimator);
 }
 
+// A token step's rotary positions, with or without the append to the KV cache, and its sampling.  Failures are the
+// LM's own, as for its norm.
+inline std::vector<double> rope_theta(int64_t rotary_dim, double base = 10000.0,
+                                      levo_rope_scaling scaling = LEVO_ROPE_SCALE_NONE, double factor = 1.0,
+                                      double context = 4096.0, double slow = 1.0, double fast = 32.0) {
+    std::vector<double> theta(static_cast<std::size_t>(rotary_dim > 1 ? rotary_dim / 2 : 1));
+    detail::check_runtime(
+        levo_rope_theta_host(theta.data(), rotary_dim, base, scaling, factor, context, slow, fast), detail::kLm);
+    return theta;
+}
+
+inline void rope_qk(const levo_rope &rope, levo_stream_t stream = nullptr) {
+    detail::check_runtime(levo_rope_qk(&rope, stream), detail::kLm);
+}
+
+inline void rope_append_kv(const levo_rope_append &append, levo_stream_t stream = nullptr) {
+    detail::check_runtime(levo_rope_append_kv(&append, stream), detail::kLm);
+}
+
+inline void sample_tokens(const levo_sampling &sampling, levo_stream_t stream = nullptr) {
+    detail::check_runtime(levo_sample_tokens(&sampling, stream), detail::kLm);
+}
+
 // combine_renderer_cfg (src/levo-renderer-pattern.cpp:123-135), device vectors.
 inline void combine_renderer_cfg(const float *unconditional, const float *conditional, float *out, int64_t n,
                                  float guidance_scale, levo_stream_t stream = nullptr) {
