@@ -666,31 +666,31 @@ def _rope_tensor(name, x, out, batch, tokens, rows, target="output"):
     shape, to = x.shape, out.shape
     if len(shape) != 4 or shape[0] != batch or shape[1] != tokens:
         raise ValueError(f"{name} must be [batch, tokens, heads, dim], its batch and tokens those of q")
-    if len(to) != 4 or to[0] != batch or to[1] != rows or to[2:] != shape[2:]:
+    if to != shape if rows == tokens else (len(to) != 4 or to[0] != batch or to[1] != rows or to[2:] != shape[2:]):
         raise ValueError(f"the {name} {target} must be [{batch}, {rows}, heads, dim] as {name} is")
     if out.dtype != x.dtype:
         raise ValueError(f"the {name} {target} must have the dtype of {name}")
     s, o = x.stride(), out.stride()
     if (s[3] != 1 or o[3] != 1) and shape[3] > 1:
         raise ValueError(f"{name} must have unit stride in its last dimension")
-    return x.data_ptr(), out.data_ptr(), shape[2], s[0], s[1], s[2], o[0], o[1], o[2]
+    return (x.data_ptr(), out.data_ptr(), shape[2], *s[:3], *o[:3])
 
 
-def _rope_args(q, theta, positions, start, flags, magnitude):
+def _rope_args(q, shape, theta, positions, start, flags, magnitude):
     """The fields of a levo_rope behind its tensors."""
     torch = _torch
     code = _dtype_of(q)
     if theta.dtype != torch.float64 or theta.dim() != 1 or not theta.is_contiguous():
         raise ValueError("theta must be a contiguous float64 [rotary_dim/2]")
-    batch, tokens, _, dim = q.shape
+    batch, tokens, _, dim = shape
     where = ps0 = ps1 = 0
     if positions is not None:
         if positions.dtype != torch.int64:
             raise ValueError("positions must be int64")
-        shape = positions.shape
-        if len(shape) == 1 and shape[0] == tokens:
+        given = positions.shape
+        if len(given) == 1 and given[0] == tokens:
             ps1 = positions.stride(0)
-        elif len(shape) == 2 and shape[0] == batch and shape[1] == tokens:
+        elif len(given) == 2 and given[0] == batch and given[1] == tokens:
             ps0, ps1 = positions.stride()
         else:
             raise ValueError("positions must be [tokens] or [batch, tokens]")
@@ -707,17 +707,18 @@ def rope_qk_t(q, k, theta, positions=None, *, start=0, interleaved=False, adjoin
     if _torch is None:
         _bind()
     torch = _torch
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError("q must be [batch, tokens, heads, dim]")
     q_out = torch.empty_like(q) if q_out is None else q_out
-    batch, tokens, _, dim = q.shape
+    batch, tokens, _, dim = shape
     k_fields = _NO_TENSOR
     if k is not None:
         if k.dtype != q.dtype or k.shape[-1] != dim:
             raise ValueError("q and k must share a dtype and a head dimension")
         k_out = torch.empty_like(k) if k_out is None else k_out
         k_fields = _rope_tensor("k", k, k_out, batch, tokens, tokens)
-    args = _rope_args(q, theta, positions, start, (ROPE_INTERLEAVED if interleaved else 0)
+    args = _rope_args(q, shape, theta, positions, start, (ROPE_INTERLEAVED if interleaved else 0)
                       | (ROPE_ADJOINT if adjoint else 0), magnitude)
     index = q.get_device()
     _same_device(index, k, theta, positions, q_out, k_out)
@@ -750,7 +751,7 @@ def rope_append_kv_t(q, k, v, theta, k_cache, v_cache, lengths, *, counts=None, 
             raise ValueError(f"{name} must be a contiguous int64 [batch]")
     if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
         raise ValueError("status must be an int32 tensor")
-    args = _rope_args(q, theta, positions, start, ROPE_INTERLEAVED if interleaved else 0, magnitude)
+    args = _rope_args(q, q.shape, theta, positions, start, ROPE_INTERLEAVED if interleaved else 0, magnitude)
     index = q.get_device()
     _same_device(index, k, v, theta, k_cache, v_cache, lengths, counts, positions, q_out, status)
     v_fields = _rope_tensor("v", v, v_cache, batch, tokens, capacity, "cache")
