@@ -156,20 +156,21 @@ __device__ __forceinline__ int turn_slot(int p, int turned_chunks) {
     return 4 * (j / 2 * turned_chunks + c) + j % 2;
 }
 
-// Two values to F32 and back, one instruction each way for the 16-bit types.
-__device__ __forceinline__ float2 to_f32x2(float x, float y) { return make_float2(x, y); }
-__device__ __forceinline__ float2 to_f32x2(__half x, __half y) { return __half22float2(__halves2half2(x, y)); }
-__device__ __forceinline__ float2 to_f32x2(__nv_bfloat16 x, __nv_bfloat16 y) {
-    return __bfloat1622float2(__halves2bfloat162(x, y));
+// Two neighbouring values to F32 and back as one word of the 16-bit types (taken apart and put together again by
+// halves they cost a 16001-token BF16 backward pass 10 %).
+__device__ __forceinline__ float2 to_f32x2(const float *p) { return *reinterpret_cast<const float2 *>(p); }
+__device__ __forceinline__ float2 to_f32x2(const __half *p) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(p));
 }
-__device__ __forceinline__ void from_f32x2(float2 v, float &x, float &y) { x = v.x, y = v.y; }
-__device__ __forceinline__ void from_f32x2(float2 v, __half &x, __half &y) {
-    const __half2 h = __floats2half2_rn(v.x, v.y);
-    x = __low2half(h), y = __high2half(h);
+__device__ __forceinline__ float2 to_f32x2(const __nv_bfloat16 *p) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(p));
 }
-__device__ __forceinline__ void from_f32x2(float2 v, __nv_bfloat16 &x, __nv_bfloat16 &y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-    x = __low2bfloat16(h), y = __high2bfloat16(h);
+__device__ __forceinline__ void from_f32x2(float2 v, float *p) { *reinterpret_cast<float2 *>(p) = v; }
+__device__ __forceinline__ void from_f32x2(float2 v, __half *p) {
+    *reinterpret_cast<__half2 *>(p) = __floats2half2_rn(v.x, v.y);
+}
+__device__ __forceinline__ void from_f32x2(float2 v, __nv_bfloat16 *p) {
+    *reinterpret_cast<__nv_bfloat162 *>(p) = __floats2bfloat162_rn(v.x, v.y);
 }
 
 // The turns of two pairs: cosines, then sines.
@@ -199,19 +200,19 @@ __device__ __forceinline__ void turn_pairs(Vec<T, VEC> (&x)[2], const Turns2 *tu
 #pragma unroll
             for (int j = i; j < i + 2; ++j) {
                 T *const pair = &x[j / (VEC / 2)].v[2 * (j % (VEC / 2))];
-                const float2 v = to_f32x2(pair[0], pair[1]);
+                const float2 v = to_f32x2(pair);
                 const float c = j > i ? t.c.y : t.c.x, s = j > i ? t.s.y : t.s.x;
-                from_f32x2(turn_pair(v.x, v.y, c, s), pair[0], pair[1]);
+                from_f32x2(turn_pair(v.x, v.y, c, s), pair);
             }
         }
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; i += 2) {
             const Turns2 t = turns[i / 2 * turned_chunks];
-            const float2 x1 = to_f32x2(x[0].v[i], x[0].v[i + 1]), x2 = to_f32x2(x[1].v[i], x[1].v[i + 1]);
+            const float2 x1 = to_f32x2(x[0].v + i), x2 = to_f32x2(x[1].v + i);
             const float2 p = __fmul2_rn(x2, t.s);
-            from_f32x2(__ffma2_rn(x1, t.c, make_float2(-p.x, -p.y)), x[0].v[i], x[0].v[i + 1]);
-            from_f32x2(__ffma2_rn(x1, t.s, __fmul2_rn(x2, t.c)), x[1].v[i], x[1].v[i + 1]);
+            from_f32x2(__ffma2_rn(x1, t.c, make_float2(-p.x, -p.y)), x[0].v + i);
+            from_f32x2(__ffma2_rn(x1, t.s, __fmul2_rn(x2, t.c)), x[1].v + i);
         }
     }
 }
@@ -248,6 +249,12 @@ __device__ __forceinline__ void copy_in(void *to, const void *from) {
 // A CTA turns a tile of tokens.  A thread keeps one chunk of one head and goes through the tile's tokens: it starts
 // the copies of all its vectors to shared memory (it alone reads them: no registers wait for them and no barrier), the
 // CTA evaluates every sine and cosine of the tile once while they are on their way, and the thread turns and stores.
+//
+// Bound by HBM on long inputs: 16001 tokens of 40 BF16 heads of 128 take 52.5 us, 6.2 TB/s (95 % of the measured copy
+// rate); 4 x 2048 tokens of 24 F16 heads 18.7 us, 5.4 TB/s (the start and end of 2048 CTAs and 220 instructions a
+// warp and 32 bytes a lane, two thirds of the issue slots); 2 x 1000 tokens of 40 F32 heads of 110, whose rows allow
+// 8 bytes an access, 16.5 us, 4.3 TB/s.  Held in registers instead of staged (two heads or tokens a thread), 4 x 2048
+// tokens took 26 to 36 us: the values on their way cost the occupancy that hides them.  One token: 3 us, the launch.
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(kMaxThreads, kCtasPerSm) rope_kernel(const RopeArgs<T> a) {
     using V = Vec<T, VEC>;
