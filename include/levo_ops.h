@@ -632,7 +632,8 @@ LEVO_OPS_API int levo_greedy_tokens_f32(const float *logits, int64_t rows, int64
 #define LEVO_ROPE_INTERLEAVED 1u
 #define LEVO_ROPE_ADJOINT 2u
 
-/* [batch][tokens][heads][head_dim]: any layout with unit stride in head_dim. */
+/* [batch][tokens][heads][head_dim]: any layout with unit stride in head_dim.
+ * Within a call no output may overlap another tensor's output or input. */
 typedef struct {
     const void *in;
     void *out;             /* may be `in` with the same strides (in place) */

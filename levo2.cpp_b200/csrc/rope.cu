@@ -528,6 +528,16 @@ int check_rope(const char *what, const levo_rope &r, size_t *element) {
     return LEVO_OPS_OK;
 }
 
+// Outputs that are another tensor's output or input: threads of both would race on them.
+int check_aliases(const char *what, const levo_rope &r, const levo_rope_tensor *v) {
+    const levo_rope_tensor *const tensors[3] = {&r.q, &r.k, v};
+    for (const levo_rope_tensor *x : tensors)
+        for (const levo_rope_tensor *y : tensors)
+            if (x && y && x != y && x->heads && y->heads && (x->out == y->out || x->out == y->in))
+                return set_error(LEVO_OPS_EINVAL, std::string(what) + ": an output is another tensor's output or input");
+    return LEVO_OPS_OK;
+}
+
 int dispatch(const levo_rope &r, const levo_rope_append *ap, const char *what, levo_stream_t stream) {
     if (r.head_dim > kMaxDim || (ap && ap->v.heads && ap->v_dim > kMaxDim))
         return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": head dimension above 8192");
@@ -560,6 +570,7 @@ LEVO_OPS_API int levo_rope_qk(const levo_rope *rope, levo_stream_t stream) {
     if ((rc = check_tensor(w, "q", r.q, r.batch, r.tokens, r.tokens, r.head_dim, element)) != LEVO_OPS_OK) return rc;
     if ((rc = check_tensor(w, "k", r.k, r.batch, r.tokens, r.tokens, r.head_dim, element)) != LEVO_OPS_OK) return rc;
     if (r.batch == 0 || r.tokens == 0 || r.q.heads + r.k.heads == 0) return LEVO_OPS_OK;
+    if ((rc = check_aliases(w, r, nullptr)) != LEVO_OPS_OK) return rc;
     return dispatch(r, nullptr, w, stream);
 }
 
@@ -586,6 +597,7 @@ LEVO_OPS_API int levo_rope_append_kv(const levo_rope_append *append, levo_stream
     if (!aligned_to(p.lengths, 8) || !aligned_to(p.counts, 8) || !aligned_to(p.status, 4))
         return fail(": pointer is not aligned to its element size");
     if (r.batch == 0 || r.tokens == 0 || r.q.heads + r.k.heads + p.v.heads == 0) return LEVO_OPS_OK;
+    if ((rc = check_aliases(w, r, &p.v)) != LEVO_OPS_OK) return rc;
     return dispatch(r, append, w, stream);
 }
 

@@ -22,7 +22,7 @@ def buf():
 def rope_args(ops, p, **changes):
     """A valid call on made-up addresses (never dereferenced: what is refused never launches)."""
     q = ops.RopeTensor(p, p + 128, 2, 32, 16, 8, 32, 16, 8)
-    k = ops.RopeTensor(p, p + 128, 2, 32, 16, 8, 32, 16, 8)
+    k = ops.RopeTensor(p, p + 256, 2, 32, 16, 8, 32, 16, 8)
     r = ops.Rope(q, k, 2, 2, 8, 8, p, None, 0, 0, 0, ops.DTYPE_F32, 0, 1.0)
     for name, value in changes.items():
         target, _, field = name.rpartition("__")
@@ -74,6 +74,19 @@ def test_rope_limits(ops, buf):
                q__out_stride_batch=1 << 20, q__out_stride_token=16)
     assert lib.levo_rope_qk(ctypes.byref(rope_args(ops, p, **far)), None) == ops.EUNSUPPORTED
     assert "too many tokens" in ops.last_error()
+
+
+def test_rope_refuses_outputs_that_are_another_tensors(ops, buf):
+    p = ctypes.addressof(buf)
+    lib = ops.lib()
+    for changes in ({"k__out": p + 128}, {"q__in_": p + 256}, {"k__in_": p + 128}):
+        assert lib.levo_rope_qk(ctypes.byref(rope_args(ops, p, **changes)), None) == ops.EINVAL
+        assert "another tensor's" in ops.last_error()
+    for out, start in ((p + 256, p), (p + 128, p), (p + 384, p + 256)):  # k's cache, q's output, v in k's cache
+        v = ops.RopeTensor(start, out, 2, 32, 16, 8, 32, 16, 8)
+        a = ops.RopeAppend(rope_args(ops, p), v, 8, 2, p, None, None)
+        assert lib.levo_rope_append_kv(ctypes.byref(a), None) == ops.EINVAL
+        assert "another tensor's" in ops.last_error()
 
 
 def test_rope_zero_sizes_are_noops(ops, buf):
