@@ -26,8 +26,8 @@
 // 1e5 others.
 //
 // A CTA's share of a row is held in shared memory as F32 and read from HBM once; a
-// share that does not fit beside a second CTA on the SM is read again from L2, by a
-// ring of cp.async copies.  Rows that are few and long are split over a cluster,
+// share that does not fit (beside a second CTA, where there are many) is read again
+// from L2, by a ring of cp.async copies.  Rows that are few and long are split over a cluster,
 // whose first CTA merges the histograms, takes the decisions and holds the lists.
 //
 // What bounds it: instruction issue, not bytes.  1024 rows of 16385 in F16 (half of
@@ -58,9 +58,8 @@ constexpr int kCountBins = 512;  // and of one of counts
 constexpr int kList = 512;
 static_assert(kList == kThreads, "a listed token a thread");
 constexpr int kMaxCluster = 8;
-// Logits that a cluster's CTA is worth.  Three rows of 16385: one CTA each 10.8 us, two 14.0, four 13.6 (the cluster's
-// barriers cost more than the shorter passes save); one row of 131072: eight CTAs 26.5 us, four 40.7.
-constexpr int kLeastShare = 16384;
+constexpr int kOneShare = 32768;  // logits that a row is split from
+constexpr int kMostHeld = 32768;  // that a CTA holds: a bit each in a thread's 64
 constexpr int kRing = 8;  // groups that a thread has on their way when it reads a row again
 constexpr int kSearches = 24;  // lists of one row: three searches with up to four further cuts each, and three more
 constexpr int64_t kMaxVocab = int64_t(1) << 17;
@@ -826,7 +825,7 @@ class Row {
             return bin_of(v) - from <= to - from && key >= low && key <= high && within(v, index);
         };
         if constexpr (HELD) {
-            static_assert(112 * 1024 / sizeof(float) <= 16 * 4 * kThreads, "a thread's fours have a bit each, their logits 64");
+            static_assert(kMostHeld <= 64 * kThreads, "a bit for each of a thread's logits");
             u64 mine = 0;
             auto held = [&](int e) {
                 const float v = buf()[e];
@@ -1273,17 +1272,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
 template <typename T>
 int launch_sample(SampleArgs &a, const char *what, cudaStream_t stream) {
     constexpr int L = 16 / sizeof(T);
-    // As many CTAs a row as the SMs (two CTAs each) take at once, each with a share that is worth it.
-    int ctas = 1;
-    while (ctas < kMaxCluster && a.rows * ctas * 2 <= 2LL * sm_count() && a.vocab / ctas >= 2 * kLeastShare) ctas *= 2;
-    a.chunk = static_cast<int>((a.vocab + ctas - 1) / ctas + 7) / 8 * 8;
-    a.words = a.recent || a.ignore ? (a.chunk + 31) / 32 + 2 : 0;
-    // A share that leaves room for two CTAs an SM is held in shared memory (192 rows of 16385: 17.0 us; read again,
-    // 29); a longer one is read again from L2 (128 rows of 131072: two CTAs a row that read again 102 us, eight that
-    // hold their shares 153: four rounds of clusters).
+    // A CTA's tables, its share of the row in shared memory, and whether that leaves room for a second CTA on the SM.
     const size_t rest = 2 * kBins * sizeof(uint32_t) + 2 * kList * sizeof(u64);
-    a.slots = (a.chunk + 2 * L + 3) / 4 * 4;
-    const bool held = rest + a.slots * sizeof(float) + sizeof(Shared) <= 112 * 1024;
+    auto chunk_of = [&](int ctas) { return static_cast<int>((a.vocab + ctas - 1) / ctas + 7) / 8 * 8; };
+    auto slots_of = [&](int ctas) { return (chunk_of(ctas) + 2 * L + 3) / 4 * 4; };
+    auto two_an_sm = [&](int ctas) { return rest + slots_of(ctas) * sizeof(float) + sizeof(Shared) <= 112 * 1024; };
+    // One CTA a row up to kOneShare logits (three rows of 16385: one CTA each 10.8 us, two 14.0, four 13.6, since a
+    // cluster's barriers cost more than its shorter passes save).  A longer row is split until its shares fit two an SM
+    // (5 rows of 50257: four CTAs each 28.3 us, two 33.7; one row of 131072: eight 26.5, four 40.7), as far as the SMs
+    // take all CTAs at once.
+    int ctas = 1;
+    while (ctas < kMaxCluster && a.rows * ctas * 2 <= 2LL * sm_count() &&
+           (ctas == 1 ? a.vocab >= kOneShare : !two_an_sm(ctas)))
+        ctas *= 2;
+    a.chunk = chunk_of(ctas);
+    a.words = a.recent || a.ignore ? (a.chunk + 31) / 32 + 2 : 0;
+    // A share that leaves room for a second CTA is held in shared memory (192 rows of 16385: 17.0 us; read again, 29),
+    // a longer one where every CTA has an SM of its own (100 rows of 20011: 18.5 us, read again 25.8; one row of 32000:
+    // 21.0 and 24.4).  Others are read again from L2 (128 rows of 131072: two CTAs a row that read again 102 us, eight
+    // that hold their shares 153, four rounds of clusters).
+    a.slots = slots_of(ctas);
+    const bool held = two_an_sm(ctas) || (a.rows * ctas <= sm_count() && a.slots <= kMostHeld);
     if (!held) a.slots = kRing * kThreads * 4;
     if (a.rows * ctas > 0x7fffffff)
         return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": too many rows for one call");

@@ -158,9 +158,11 @@ def test_sample_clusters_of_close_logits(ops, dev):
     check(ops, dev, base, uniforms(gen, 6), temperature=1e6, top_p=0.3)
 
 
-# Rows x vocabulary by how a row is worked on: one CTA that holds it (few rows, many); one that reads it again; a
-# cluster of eight that holds its shares (few rows, many); clusters of two and four that read them again; one list.
-SHARES = [(7, 16385), (2, 131072), (5, 50257), (200, 16385), (300, 20011), (30, 131072), (40, 131071), (9, 512)]
+# Rows x vocabulary by how a row is worked on: one CTA that holds it (few rows, many, a long row); one that reads it
+# again; a cluster of eight that holds its shares (few rows, many), of four; one of four that reads them again, and of
+# two; one list.
+SHARES = [(7, 16385), (200, 16385), (6, 32700), (300, 20011), (2, 131072), (30, 131072), (5, 50257), (40, 131071),
+          (100, 50257), (9, 512)]
 
 
 @pytest.mark.parametrize("rows,vocab", SHARES)
