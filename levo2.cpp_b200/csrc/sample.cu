@@ -53,6 +53,7 @@ typedef unsigned long long u64;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+static_assert(kWarps <= 32 && (kWarps & (kWarps - 1)) == 0, "a warp's lanes read all warps' values");
 constexpr int kBins = 4096;      // slices of a histogram of weights
 constexpr int kCountBins = 512;  // and of one of counts
 constexpr int kList = 512;
@@ -157,7 +158,7 @@ struct Found {
 
 struct Shared {
     double powers[kSteps];
-    u64 warp_sums[kWarps];
+    u64 warp_sums[kWarps];            // of a running sum; at first each warp's largest and smallest key
     u64 total;                        // first CTA: of the histogram
     u64 passing[kMaxCluster];         // first CTA: weight that min-p leaves, of each CTA
     Found found;
@@ -170,8 +171,7 @@ struct Shared {
     uint32_t most[kMaxCluster], least[kMaxCluster], ties[kMaxCluster];  // of every CTA, in every CTA
     int nan[kMaxCluster];
     uint32_t block_most, block_least;
-    int block_nan;
-    int warp_counts[kWarps];
+    int warp_counts[kWarps];          // at first whether a warp has met a NaN
     int places[kThreads], ends[kThreads];  // of a list's slices
 };
 
@@ -208,7 +208,6 @@ class Row {
         row = row_index;
         if (tid < kSearches) sh.cursor[tid] = 0;
         if (tid < kSteps) sh.powers[tid] = kStepPowers.v[tid];
-        if (tid == 0) sh.block_most = 0, sh.block_least = 0xffffffffu, sh.block_nan = 0;
         ask();
         load();
         share_extremes();
@@ -458,27 +457,30 @@ class Row {
         const uint32_t most_key = __reduce_max_sync(0xffffffffu, key_of(most));
         const uint32_t least_key = __reduce_min_sync(0xffffffffu, key_of(least));
         nan = __any_sync(0xffffffffu, nan);
+        // a place of its own for each warp: this barrier may be the kernel's first, so nothing could be set before it
         if ((tid & 31) == 0) {
-            atomicMax(&sh.block_most, most_key);
-            atomicMin(&sh.block_least, least_key);
-            if (nan) sh.block_nan = 1;
+            sh.warp_sums[tid >> 5] = (static_cast<u64>(most_key) << 32) | least_key;
+            sh.warp_counts[tid >> 5] = nan;
         }
         __syncthreads();
     }
 
-    // Largest and smallest key (and the NaN flag) of the row, from those of each CTA.
+    // Largest and smallest key (and the NaN flag) of the row, from those of each warp and each CTA.
     __device__ __forceinline__ void share_extremes() {
+        const int warp = tid & (kWarps - 1);
+        uint32_t most = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(sh.warp_sums[warp] >> 32));
+        uint32_t least = __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(sh.warp_sums[warp]));
+        const int nan = __any_sync(0xffffffffu, sh.warp_counts[warp]);
         if (CLUSTER) {
             if (tid < ctas) {
-                *at(&sh.most[rank], tid) = sh.block_most;
-                *at(&sh.least[rank], tid) = sh.block_least;
-                *at(&sh.nan[rank], tid) = sh.block_nan;
+                *at(&sh.most[rank], tid) = most;
+                *at(&sh.least[rank], tid) = least;
+                *at(&sh.nan[rank], tid) = nan;
             }
             sync_all();
         } else if (tid == 0) {
-            sh.nan[0] = sh.block_nan;
+            sh.nan[0] = nan;
         }
-        uint32_t most = sh.block_most, least = sh.block_least;
         if (CLUSTER)
             for (int i = 0; i < ctas; ++i) most = max(most, sh.most[i]), least = min(least, sh.least[i]);
         top = value_of(most);

@@ -396,3 +396,30 @@ def test_sample_on_a_device_that_is_not_current(ops, dev):
 
 def test_sample_no_rows(ops, dev):
     assert ops.sample_tokens_t(torch.empty((0, 10), device=dev), torch.empty(0, device=dev)).shape == (0,)
+
+
+# Vocabularies that one CTA reads: held, read again with many rows of two CTAs an SM, in one or several rounds of loads.
+@pytest.mark.parametrize("rows,vocab", [(160, 16384), (160, 2048), (320, 20480)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_sample_extremes_in_every_warps_share(ops, dev, dtype, rows, vocab):
+    """Rows without edited ids: the largest and the smallest logit, and a NaN, in the share of each warp in turn
+    (a thread reads 16 bytes, a warp 512, sixteen warps one after the other), whichever warp comes first."""
+    gen = torch.Generator(device=dev).manual_seed(vocab)
+    t = DTYPES[dtype]
+    of_warp = 512 // torch.empty(0, dtype=t).element_size()
+    x = torch.randn((rows, vocab), generator=gen, device=dev).to(t)
+    r = torch.arange(rows, device=dev)
+    inside = torch.randint(0, of_warp, (2, rows), generator=gen, device=dev)
+    most = (r % 16 * of_warp + inside[0]) % vocab
+    least = ((r // 16 + r + 5) % 16 * of_warp + inside[1]) % vocab
+    x[r, least] = -9.0
+    x[r, most] = 9.0
+    for name in ("none", "k50", "p50", "m0.1", "hot", "zero"):
+        check(ops, dev, x, uniforms(gen, rows), **FILTERS[name])
+    # a NaN in one row: the flag, and the token of the others
+    for row in range(0, 32, 3):
+        y = x.clone()
+        y[row, least[row]] = math.nan
+        status = torch.zeros(1, dtype=torch.int32, device=dev)
+        tokens = ops.sample_tokens_t(y, uniforms(gen, rows), temperature=0.0, status=status)
+        assert status.item() == ops.SAMPLE_NAN and torch.equal(tokens, most)
