@@ -205,6 +205,9 @@ class Row {
     }
 
     __device__ __forceinline__ void run(int64_t row_index) {
+        // Shared memory of another CTA may be touched once that CTA runs: all of the cluster's arrive here, and wait for
+        // one another behind the load.
+        if (CLUSTER) cg::this_cluster().barrier_arrive();
         row = row_index;
         if (tid < kSearches) sh.cursor[tid] = 0;
         if (tid < kSteps) sh.powers[tid] = kStepPowers.v[tid];
@@ -472,6 +475,7 @@ class Row {
         uint32_t least = __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(sh.warp_sums[warp]));
         const int nan = __any_sync(0xffffffffu, sh.warp_counts[warp]);
         if (CLUSTER) {
+            cg::this_cluster().barrier_wait();
             if (tid < ctas) {
                 *at(&sh.most[rank], tid) = most;
                 *at(&sh.least[rank], tid) = least;

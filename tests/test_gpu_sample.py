@@ -423,3 +423,28 @@ def test_sample_extremes_in_every_warps_share(ops, dev, dtype, rows, vocab):
         status = torch.zeros(1, dtype=torch.int32, device=dev)
         tokens = ops.sample_tokens_t(y, uniforms(gen, rows), temperature=0.0, status=status)
         assert status.item() == ops.SAMPLE_NAN and torch.equal(tokens, most)
+
+
+@pytest.mark.parametrize("rows,vocab", [(18, 32768), (37, 32800), (18, 131072), (60, 50257)])
+def test_sample_split_rows_behind_and_beside_other_work(ops, dev, rows, vocab):
+    """CTAs of a cluster that start late and read little: behind products that fill the SMs, on several streams at
+    once, with nothing to edit and with everything masked but a share's end."""
+    gen = torch.Generator(device=dev).manual_seed(rows + vocab)
+    x = (2 * torch.randn((rows, vocab), generator=gen, device=dev)).bfloat16()
+    x[0, :-1] = -math.inf
+    x[1, 1:] = -math.inf
+    u = uniforms(gen, rows)
+    want = torch.from_numpy(check(ops, dev, x, u, top_p=0.9))
+    a = torch.randn((2048, 2048), generator=gen, device=dev)
+    streams = [torch.cuda.Stream(device=dev) for _ in range(3)]
+    for stream in streams:
+        stream.wait_stream(torch.cuda.current_stream(dev))
+    results = []
+    for _ in range(20):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                a @ a
+                results += [ops.sample_tokens_t(x, u, top_p=0.9) for _ in range(2)]
+    torch.cuda.synchronize()
+    for tokens in results:
+        assert torch.equal(tokens.cpu(), want)
