@@ -151,6 +151,12 @@ struct Settings {
     int bad;
 };
 
+// Largest and smallest key, and whether there is a NaN.
+struct Extremes {
+    uint32_t most, least;
+    int nan;
+};
+
 // A token found: its place in the order, what lies before it, and what it has itself (weight, or 1).
 struct Found {
     u64 order, before, own;
@@ -168,8 +174,9 @@ struct Shared {
     int joint;                        // it is
     Settings set;
     int cursor[kSearches];            // first CTA: tokens of each list
+    Extremes own;                     // of this CTA's share
+    int nan;                          // the row has a NaN
     uint32_t most[kMaxCluster], least[kMaxCluster], ties[kMaxCluster];  // of every CTA, in every CTA
-    int nan[kMaxCluster];
     uint32_t block_most, block_least;
     int warp_counts[kWarps];          // at first whether a warp has met a NaN
     int places[kThreads], ends[kThreads];  // of a list's slices
@@ -205,9 +212,6 @@ class Row {
     }
 
     __device__ __forceinline__ void run(int64_t row_index) {
-        // Shared memory of another CTA may be touched once that CTA runs: all of the cluster's arrive here, and wait for
-        // one another behind the load.
-        if (CLUSTER) cg::this_cluster().barrier_arrive();
         row = row_index;
         if (tid < kSearches) sh.cursor[tid] = 0;
         if (tid < kSteps) sh.powers[tid] = kStepPowers.v[tid];
@@ -473,20 +477,18 @@ class Row {
         const int warp = tid & (kWarps - 1);
         uint32_t most = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(sh.warp_sums[warp] >> 32));
         uint32_t least = __reduce_min_sync(0xffffffffu, static_cast<uint32_t>(sh.warp_sums[warp]));
-        const int nan = __any_sync(0xffffffffu, sh.warp_counts[warp]);
+        int nan = __any_sync(0xffffffffu, sh.warp_counts[warp]);
         if (CLUSTER) {
-            cg::this_cluster().barrier_wait();
-            if (tid < ctas) {
-                *at(&sh.most[rank], tid) = most;
-                *at(&sh.least[rank], tid) = least;
-                *at(&sh.nan[rank], tid) = nan;
-            }
+            // Another CTA's shared memory may be touched once that CTA runs, which this barrier, the first, is what says:
+            // so each leaves its own for the others to fetch.
+            if (tid == 0) sh.own = {most, least, nan};
             sync_all();
-        } else if (tid == 0) {
-            sh.nan[0] = nan;
+            const Extremes theirs = *at(&sh.own, min(tid & 31, ctas - 1));
+            most = __reduce_max_sync(0xffffffffu, theirs.most);
+            least = __reduce_min_sync(0xffffffffu, theirs.least);
+            nan = __any_sync(0xffffffffu, theirs.nan);
         }
-        if (CLUSTER)
-            for (int i = 0; i < ctas; ++i) most = max(most, sh.most[i]), least = min(least, sh.least[i]);
+        if (tid == 0) sh.nan = nan;
         top = value_of(most);
         lowest = value_of(least);
     }
@@ -1263,7 +1265,7 @@ class Row {
     }
     __device__ __forceinline__ void flag(int flags) {
         if (sh.set.bad) flags |= LEVO_SAMPLE_PARAM;
-        for (int c = 0; c < ctas; ++c) flags |= sh.nan[c] ? LEVO_SAMPLE_NAN : 0;
+        if (sh.nan) flags |= LEVO_SAMPLE_NAN;
         if (a.status && flags) atomicOr(a.status, flags);
     }
 };
