@@ -62,6 +62,8 @@ constexpr int kMaxCluster = 8;
 constexpr int kOneShare = 32768;  // logits that a row is split from
 constexpr int kMostHeld = 32768;  // that a CTA holds: a bit each in a thread's 64
 constexpr int kRing = 8;  // groups that a thread has on their way when it reads a row again
+// Slices are at least 2^-128 of (top - v) / 2 wide, so from 15.95 T = 2^-116 down kBins of them end beyond the weights.
+constexpr float kTinyTemperature = 1e-36f;
 constexpr int kSearches = 24;  // lists of one row: three searches with up to four further cuts each, and three more
 constexpr int64_t kMaxVocab = int64_t(1) << 17;
 
@@ -121,7 +123,7 @@ struct StepPowers {
 };
 __device__ const StepPowers kStepPowers{};
 
-// For v within 32 T of the top, as bin_of takes them: the result is below 2^45 and its exponent above -3.
+// For v within 32 T of the top, as bin_of and `seen` take them: the result is below 2^45 and its exponent above -3.
 __device__ __forceinline__ u64 weight_of(float v, double top, double scale, const double *powers) {
     const double y = (static_cast<double>(v) - top) * scale;
     constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
@@ -263,7 +265,7 @@ class Row {
     float half_top, reach, slices;   // slices of a unit of (top - v) / 2, which has weight up to `reach`
     int bins;
     double wide_top, scale;
-    bool infinite;
+    enum { kPlain, kInfinite, kTiny } special;  // whether, and how, logits are not taken as they are
     bool limited = false;  // by top-k: tokens up to (limit_value, limit_index) in the order
     float limit_value;
     int limit_index;
@@ -514,16 +516,21 @@ class Row {
     __device__ __forceinline__ void settings() {
         const float temperature = sh.set.temperature;
         scale = temperature > 0.0f ? kSteps * 1.4426950408889634074 / static_cast<double>(temperature) : 0.0;
-        infinite = top == INFINITY;  // +inf alone has weight: as 0 among -inf
-        if (infinite) {
-            top = lowest = 0.0f;
-            thread_top = thread_top == INFINITY ? 0.0f : -INFINITY;
-        }
+        special = top == INFINITY ? kInfinite : temperature > 0.0f && temperature < kTinyTemperature ? kTiny : kPlain;
+        if (special == kInfinite) top = lowest = 0.0f;
         // Half differences, so that none overflows.  The slices reach to the lowest logit, or to 31.9 T below the top,
         // where weights are below 2^-45 and round to nothing.
         half_top = 0.5f * top;
         wide_top = top;
         reach = fminf(__fmaf_rn(-0.5f, lowest, half_top), 15.95f * temperature);
+        if (special) thread_top = seen(thread_top);
+    }
+
+    // A logit of a special row.  Beside +inf nothing else has weight: 0 among -inf.  At a tiny temperature the slices
+    // would take in logits thousands of temperatures below the top: those are -inf.
+    __device__ __forceinline__ float seen(float v) const {
+        if (special == kInfinite) return v == INFINITY ? 0.0f : -INFINITY;
+        return static_cast<double>(v) - wide_top >= -32.0 * static_cast<double>(sh.set.temperature) ? v : -INFINITY;
     }
 
     // Slice of a logit: never smaller for a smaller logit; `bins` and above where there is no weight (-inf among it)
@@ -560,9 +567,9 @@ class Row {
     template <typename F>
     __device__ __forceinline__ void for_fours(F f) {
         auto four = [&](float(&v)[4], int first) {
-            if (infinite) {
+            if (special) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = v[i] == INFINITY ? 0.0f : -INFINITY;
+                for (int i = 0; i < 4; ++i) v[i] = seen(v[i]);
             }
             f(v, first);
         };
@@ -837,7 +844,7 @@ class Row {
             u64 mine = 0;
             auto held = [&](int e) {
                 const float v = buf()[e];
-                return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
+                return special ? seen(v) : v;
             };
             for (; quads != 0; quads &= quads - 1) {
                 const int quad = __ffs(quads) - 1, e = 4 * (tid + quad * kThreads);
@@ -1057,7 +1064,7 @@ class Row {
     }
     __device__ __forceinline__ float logit(int i) const {
         const float v = raw_logit(i);
-        return infinite ? (v == INFINITY ? 0.0f : -INFINITY) : v;
+        return special ? seen(v) : v;
     }
 
     // Index of this CTA's n-th (from 0) token with that logit: in the thread that holds it, -1 in the others.

@@ -448,3 +448,22 @@ def test_sample_split_rows_behind_and_beside_other_work(ops, dev, rows, vocab):
     torch.cuda.synchronize()
     for tokens in results:
         assert torch.equal(tokens.cpu(), want)
+
+
+@pytest.mark.parametrize("rows,vocab", [(7, 16385), (200, 5000), (300, 20011), (7, 131072), (9, 512)])
+@pytest.mark.parametrize("temperature", [1e-30, 1e-36, 1e-37, 3e-38, 1e-38, 1e-41, 1e-45])
+def test_sample_tiny_temperatures(ops, dev, rows, vocab, temperature):
+    """Logits so near the top that a temperature below F32's normal range still tells them apart, and others that
+    lie thousands of temperatures below it: those have no weight, whatever slice they fall into."""
+    rng = np.random.default_rng(rows + vocab)
+    x = np.zeros((rows, vocab), np.float64)
+    for r in range(rows):
+        near = rng.random(vocab)
+        x[r] = (-2.3e-35 * near, -300 * temperature * near, 3e-36 * near, -2.0 ** -149 * rng.integers(0, 9000, vocab),
+                np.floor(4 * near), np.where(near < 0.5, -40 * temperature * near, -3e38),
+                np.where(near < 0.01, -3 * temperature * rng.random(vocab), -2.4e-35 * near))[r % 7]
+    x[5::7, ::3] = -np.inf
+    logits = torch.from_numpy(x.astype(np.float32)).to(dev)
+    gen = torch.Generator(device=dev).manual_seed(vocab)
+    for name in ("none", "k50", "k1500", "p50", "p999", "m0.1", "k+p"):
+        check(ops, dev, logits, uniforms(gen, rows), temperature=temperature, **FILTERS[name])
