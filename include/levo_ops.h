@@ -633,7 +633,8 @@ LEVO_OPS_API int levo_greedy_tokens_f32(const float *logits, int64_t rows, int64
 #define LEVO_ROPE_ADJOINT 2u
 
 /* [batch][tokens][heads][head_dim]: any layout with unit stride in head_dim.
- * Within a call no output may overlap another tensor's output or input. */
+ * A call whose outputs share an element with another tensor's output or input, or
+ * with their own input but in place, is refused. */
 typedef struct {
     const void *in;
     void *out;             /* may be `in` with the same strides (in place) */
@@ -683,7 +684,8 @@ LEVO_OPS_API int levo_rope_theta_host(double *theta_host, int64_t rotary_dim, do
  *   k.out[b][lengths[b] + s] = k turned, v.out[b][lengths[b] + s] = v    for s < counts[b],
  *   q.out[b][s]              = q turned                                  for every s.
  * The caches are [batch][capacity][heads][dim] by k.out_stride / v.out_stride; every other
- * row of theirs is left as it was.  Positions default to lengths[b] + s (+ rope.start).
+ * row of theirs is left as it was.  k.in and v.in lie outside their caches, or, in a call of
+ * one token, on a row of them.  Positions default to lengths[b] + s (+ rope.start).
  * lengths and counts lie on the device, so a captured graph serves every step: the caller
  * advances them.  A sequence's lengths are the same for all layers of a step and are not written.
  * rope.flags may not hold LEVO_ROPE_ADJOINT.

@@ -18,6 +18,7 @@
 #include <cmath>
 
 #include "common.cuh"
+#include "strided.h"
 
 namespace levo {
 namespace {
@@ -464,21 +465,13 @@ constexpr int64_t kMaxDim = 2 * kMaxTurns;      // a token's sines and cosines f
 constexpr int64_t kMaxSpan = int64_t(1) << 60;  // of a stride times its size
 constexpr double kMaxWork = 1e16;               // values of one call: its counters stay inside 64 bits
 
-// Whether [n0][n1][n2][inner] by these strides names distinct elements, and by how much it spans
-// (sorted by stride, each dimension steps past all that the smaller ones reach).
-bool distinct_elements(const int64_t (&stride)[3], const int64_t (&size)[3], int64_t inner) {
-    int64_t reach = inner;
-    bool done[3] = {false, false, false};
-    for (int round = 0; round < 3; ++round) {
-        int least = -1;
-        for (int i = 0; i < 3; ++i)
-            if (!done[i] && (least < 0 || stride[i] < stride[least])) least = i;
-        done[least] = true;
-        if (size[least] <= 1) continue;
-        if (stride[least] < reach) return false;
-        reach += stride[least] * (size[least] - 1);
-    }
-    return true;
+Strided input_of(const levo_rope_tensor &t, int64_t batch, int64_t tokens, int64_t dim) {
+    return {reinterpret_cast<uintptr_t>(t.in), {t.in_stride[0], t.in_stride[1], t.in_stride[2]},
+            {batch, tokens, t.heads}, dim};
+}
+Strided output_of(const levo_rope_tensor &t, int64_t batch, int64_t rows, int64_t dim) {
+    return {reinterpret_cast<uintptr_t>(t.out), {t.out_stride[0], t.out_stride[1], t.out_stride[2]},
+            {batch, rows, t.heads}, dim};
 }
 
 int check_tensor(const char *what, const char *name, const levo_rope_tensor &t, int64_t batch, int64_t tokens,
@@ -498,7 +491,7 @@ int check_tensor(const char *what, const char *name, const levo_rope_tensor &t, 
             t.out_stride[i] > kMaxSpan / std::max<int64_t>(out_size[i], 1))
             return fail(": stride too large");
     }
-    if (!distinct_elements(t.out_stride, out_size, dim)) return fail(": the output's strides overlap");
+    if (!output_of(t, batch, rows, dim).distinct()) return fail(": the output's strides overlap");
     if (t.in == t.out && rows == tokens) {
         for (int i = 0; i < 3; ++i)
             if (in_size[i] > 1 && t.in_stride[i] != t.out_stride[i])
@@ -528,23 +521,52 @@ int check_rope(const char *what, const levo_rope &r, size_t *element) {
     return LEVO_OPS_OK;
 }
 
-// Outputs that are another tensor's output or input: threads of both would race on them.
-int check_aliases(const char *what, const levo_rope &r, const levo_rope_tensor *v) {
-    const levo_rope_tensor *const tensors[3] = {&r.q, &r.k, v};
-    for (const levo_rope_tensor *x : tensors)
-        for (const levo_rope_tensor *y : tensors)
-            if (x && y && x != y && x->heads && y->heads && (x->out == y->out || x->out == y->in))
-                return set_error(LEVO_OPS_EINVAL, std::string(what) + ": an output is another tensor's output or input");
+// Whether one token's input lies exactly on a row of its own cache: whatever row the token goes to, each thread reads
+// and writes its own values of a head.
+bool on_a_row(const Strided &in, const Strided &cache, size_t element) {
+    for (int i : {0, 2})
+        if (in.size[i] > 1 && in.stride[i] != cache.stride[i]) return false;
+    const uintptr_t apart = (in.at - cache.at) / element;
+    const int64_t rows = cache.size[1];
+    return in.size[1] == 1 && rows > 1 && in.at >= cache.at && apart % static_cast<uintptr_t>(cache.stride[1]) == 0 &&
+           apart / static_cast<uintptr_t>(cache.stride[1]) < static_cast<uintptr_t>(rows);
+}
+
+// Outputs that share elements with another tensor's output or input, or with their own input but in place: threads
+// would race on them.
+int check_overlaps(const char *what, const levo_rope &r, const levo_rope_append *ap, size_t element) {
+    auto fail = [&](const char *why) { return set_error(LEVO_OPS_EINVAL, std::string(what) + why); };
+    const levo_rope_tensor *const tensors[3] = {&r.q, &r.k, ap ? &ap->v : nullptr};
+    Strided in[3], out[3];
+    int n = 0;
+    for (int i = 0; i < 3; ++i) {
+        const levo_rope_tensor *const t = tensors[i];
+        if (!t || !t->heads) continue;
+        const int64_t dim = i == 2 ? ap->v_dim : r.head_dim;
+        in[n] = input_of(*t, r.batch, r.tokens, dim);
+        out[n++] = output_of(*t, r.batch, ap && i > 0 ? ap->capacity : r.tokens, dim);
+    }
+    for (int i = 0; i < n; ++i)
+        for (int j = 0; j < n; ++j)
+            if (i != j && ((i < j && overlap(out[i], out[j], element)) || overlap(out[i], in[j], element)))
+                return fail(": an output overlaps another tensor's output or input");
+    for (int i = 0; i < n; ++i) {
+        if (in[i].at == out[i].at && in[i].size[1] == out[i].size[1]) continue;  // in place: check_tensor saw the strides
+        if (overlap(out[i], in[i], element) && !on_a_row(in[i], out[i], element))
+            return fail(": an output overlaps its own input and is not in place");
+    }
     return LEVO_OPS_OK;
 }
 
-int dispatch(const levo_rope &r, const levo_rope_append *ap, const char *what, levo_stream_t stream) {
+int dispatch(const levo_rope &r, const levo_rope_append *ap, size_t element, const char *what, levo_stream_t stream) {
     if (r.head_dim > kMaxDim || (ap && ap->v.heads && ap->v_dim > kMaxDim))
         return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": head dimension above 8192");
     const double width = static_cast<double>(std::max(r.head_dim, ap ? ap->v_dim : 0));
     const double heads = static_cast<double>(r.q.heads + r.k.heads + (ap ? ap->v.heads : 0));
     if (static_cast<double>(r.batch) * static_cast<double>(r.tokens) * heads * width > kMaxWork)
         return set_error(LEVO_OPS_EUNSUPPORTED, std::string(what) + ": too many values for one call");
+    const int rc = check_overlaps(what, r, ap, element);
+    if (rc != LEVO_OPS_OK) return rc;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (r.dtype == LEVO_DTYPE_F32) return launch_rope<float>(r, ap, what, s);
     if (r.dtype == LEVO_DTYPE_F16) return launch_rope<__half>(r, ap, what, s);
@@ -570,8 +592,7 @@ LEVO_OPS_API int levo_rope_qk(const levo_rope *rope, levo_stream_t stream) {
     if ((rc = check_tensor(w, "q", r.q, r.batch, r.tokens, r.tokens, r.head_dim, element)) != LEVO_OPS_OK) return rc;
     if ((rc = check_tensor(w, "k", r.k, r.batch, r.tokens, r.tokens, r.head_dim, element)) != LEVO_OPS_OK) return rc;
     if (r.batch == 0 || r.tokens == 0 || r.q.heads + r.k.heads == 0) return LEVO_OPS_OK;
-    if ((rc = check_aliases(w, r, nullptr)) != LEVO_OPS_OK) return rc;
-    return dispatch(r, nullptr, w, stream);
+    return dispatch(r, nullptr, element, w, stream);
 }
 
 LEVO_OPS_API int levo_rope_append_kv(const levo_rope_append *append, levo_stream_t stream) {
@@ -591,14 +612,13 @@ LEVO_OPS_API int levo_rope_append_kv(const levo_rope_append *append, levo_stream
     if ((rc = check_tensor(w, "q", r.q, r.batch, r.tokens, r.tokens, r.head_dim, element)) != LEVO_OPS_OK) return rc;
     if ((rc = check_tensor(w, "k", r.k, r.batch, r.tokens, p.capacity, r.head_dim, element)) != LEVO_OPS_OK) return rc;
     if ((rc = check_tensor(w, "v", p.v, r.batch, r.tokens, p.capacity, p.v_dim, element)) != LEVO_OPS_OK) return rc;
-    if ((r.k.heads && r.k.in == r.k.out) || (p.v.heads && p.v.in == p.v.out))
+    if (r.tokens > 1 && ((r.k.heads && r.k.in == r.k.out) || (p.v.heads && p.v.in == p.v.out)))
         return fail(": a cache may not be its own input");
     if (p.lengths == nullptr) return fail(": lengths is null");
     if (!aligned_to(p.lengths, 8) || !aligned_to(p.counts, 8) || !aligned_to(p.status, 4))
         return fail(": pointer is not aligned to its element size");
     if (r.batch == 0 || r.tokens == 0 || r.q.heads + r.k.heads + p.v.heads == 0) return LEVO_OPS_OK;
-    if ((rc = check_aliases(w, r, &p.v)) != LEVO_OPS_OK) return rc;
-    return dispatch(r, append, w, stream);
+    return dispatch(r, append, element, w, stream);
 }
 
 LEVO_OPS_API int levo_rope_theta_host(double *theta_host, int64_t rotary_dim, double base, int32_t scaling,

@@ -338,3 +338,55 @@ def test_rope_random_layouts(ops, dev, seed):
     theta = ops.rope_theta(rot, device=dev)
     check_qk(ops, q, k, theta, positions, t, interleaved=bool(seed & 1), adjoint=bool(seed & 2),
              magnitude=float(rng.choice([1.0, 0.9])))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_in_place_in_a_fused_projection(ops, dev, dtype, interleaved):
+    """q and k turned where they lie between one another and v; and a step into the free rows between."""
+    gen = torch.Generator(device=dev).manual_seed(13)
+    t, b, s, hq, hk, d = DTYPES[dtype], 2, 23, 4, 2, 64
+    fused = make(gen, (b, s, hq + 2 * hk, d), t)
+    before = fused.clone()
+    theta = ops.rope_theta(d, device=dev)
+    q, k = fused[:, :, :hq], fused[:, :, hq:hq + hk]
+    want_q, want_k = ops.rope_qk_t(before[:, :, :hq], before[:, :, hq:hq + hk], theta, start=3, interleaved=interleaved)
+    ops.rope_qk_t(q, k, theta, start=3, interleaved=interleaved, q_out=q, k_out=k)
+    assert torch.equal(q, want_q) and torch.equal(k, want_k) and torch.equal(fused[:, :, hq + hk:], before[:, :, hq + hk:])
+    rows = make(gen, (b, 2 * s, hq, d), t)
+    before = rows.clone()
+    ops.rope_qk_t(rows[:, ::2], None, theta, interleaved=interleaved, q_out=rows[:, 1::2])
+    assert torch.equal(rows[:, 1::2], ops.rope_qk_t(before[:, ::2], None, theta, interleaved=interleaved)[0])
+    assert torch.equal(rows[:, ::2], before[:, ::2])
+
+
+def test_append_of_a_token_that_lies_in_its_cache(ops, dev):
+    """A projection may write a token's k and v to a row of the caches themselves; the append turns k and takes both
+    to the sequence's row, which may be that one."""
+    gen = torch.Generator(device=dev).manual_seed(14)
+    b, h, d, capacity, t = 3, 2, 64, 9, torch.float16
+    theta = ops.rope_theta(d, device=dev)
+    q = make(gen, (b, 1, h, d), t)
+    kc, vc = cache_pair(gen, b, capacity, h, d, h, d, t)
+    kt, vt = kc.clone(), vc.clone()
+    lengths = torch.tensor([5, 0, 8], device=dev)
+    for row in (5, 0, 8):
+        got = ops.rope_append_kv_t(q, kc[:, row:row + 1], vc[:, row:row + 1], theta, kc, vc, lengths)
+        want = ops.rope_append_kv_t(q, kt[:, row:row + 1].clone(), vt[:, row:row + 1].clone(), theta, kt, vt, lengths)
+        assert torch.equal(got, want) and torch.equal(kc, kt) and torch.equal(vc, vt)
+
+
+def test_rope_refuses_overlapping_views(ops, dev):
+    theta = ops.rope_theta(16, device=dev)
+    big = torch.zeros((2, 7, 3, 16), device=dev)
+    with pytest.raises(ValueError, match="its own input"):
+        ops.rope_qk_t(big[:, :-1], None, theta, q_out=big[:, 1:])
+    with pytest.raises(ValueError, match="another tensor's"):
+        ops.rope_qk_t(torch.zeros((2, 5, 3, 16), device=dev), big[:, :5], theta, q_out=big[:, 2:])
+    lengths = torch.zeros(2, dtype=torch.int64, device=dev)
+    q = torch.zeros((2, 3, 3, 16), device=dev)
+    with pytest.raises(ValueError, match="its own input"):
+        ops.rope_append_kv_t(q, big[:, 1:4], q.clone(), theta, big, big.clone(), lengths)
+    with pytest.raises(ValueError, match="another tensor's"):
+        ops.rope_append_kv_t(q, q, q, theta, big[:, :6], big[:, 1:], lengths)
+    assert int(torch.count_nonzero(big)) == 0

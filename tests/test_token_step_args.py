@@ -89,6 +89,63 @@ def test_rope_refuses_outputs_that_are_another_tensors(ops, buf):
         assert "another tensor's" in ops.last_error()
 
 
+def apart_args(ops, p):
+    """A valid call whose tensors lie apart: 256 bytes each, from 4096 bytes on."""
+    q = ops.RopeTensor(p + 4096, p + 8192, 2, 32, 16, 8, 32, 16, 8)
+    k = ops.RopeTensor(p + 12288, p + 16384, 2, 32, 16, 8, 32, 16, 8)
+    return rope_args(ops, p, q=q, k=k)
+
+
+@pytest.mark.parametrize("changes,message", [
+    ({"q__out": 4096 + 4}, "its own input"),            # one element on
+    ({"q__out": 4096 - 64}, "its own input"),           # out = buf[:, :-1], in = buf[:, 1:]
+    ({"q__out": 4096 + 252}, "its own input"),          # the last element alone
+    ({"q__out": 4096 - 252}, "its own input"),
+    ({"q__out": 4096 + 32, "q__in_stride_head": 16, "q__in_stride_token": 32, "q__in_stride_batch": 64,
+      "q__out_stride_head": 32, "q__out_stride_token": 8, "q__out_stride_batch": 64}, "its own input"),
+    ({"q__out": 4096 + 28, "q__in_stride_batch": 0, "q__in_stride_token": 0, "q__in_stride_head": 0}, "its own input"),
+    ({"k__out": 8192 + 252}, "another tensor's"), ({"k__out": 4096 - 252}, "another tensor's"),
+    ({"q__out": 12288 + 128}, "another tensor's"),
+    ({"k__in_": 8192 + 32, "k__in_stride_head": 0}, "another tensor's"),
+])
+def test_rope_refuses_outputs_that_overlap(ops, buf, changes, message):
+    p = ctypes.addressof(buf)
+    r = apart_args(ops, p)
+    for name, value in changes.items():
+        target, _, field = name.rpartition("__")
+        setattr(getattr(r, target), field, p + value if field in ("in_", "out") else value)
+    assert ops.lib().levo_rope_qk(ctypes.byref(r), None) == ops.EINVAL
+    assert message in ops.last_error(), ops.last_error()
+
+
+def test_append_refuses_caches_that_overlap(ops, buf):
+    p = ctypes.addressof(buf)
+    for k_in, k_out, v_in, v_out, message in (
+            (12288, 12288 - 64, 20480, 24576, "its own input"),     # tokens that lie in rows 1 and 2 of the cache
+            (12288, 16384, 20480, 20480 - 64, "its own input"),
+            (12288, 16384, 20480, 16384 + 508, "another tensor's"),  # the caches' ends
+            (12288, 16384, 16384 + 64, 24576, "another tensor's"),   # v in a row of k's cache
+            (12288, 8192 + 32, 20480, 24576, "another tensor's")):
+        r = apart_args(ops, p)
+        r.k = ops.RopeTensor(p + k_in, p + k_out, 2, 32, 16, 8, 64, 16, 8)
+        v = ops.RopeTensor(p + v_in, p + v_out, 2, 32, 16, 8, 64, 16, 8)
+        a = ops.RopeAppend(r, v, 8, 4, p, None, None)
+        assert ops.lib().levo_rope_append_kv(ctypes.byref(a), None) == ops.EINVAL
+        assert message in ops.last_error(), ops.last_error()
+
+
+def test_which_layouts_overlap(tmp_path):
+    """csrc/strided.h against sets of elements."""
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no host compiler")
+    exe = tmp_path / "strided"
+    subprocess.run([gxx, "-std=c++17", "-O2", "-I", str(ROOT / "levo2.cpp_b200" / "csrc"),
+                    str(ROOT / "tests" / "cpp" / "strided_test.cpp"), "-o", str(exe)], check=True)
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and "strided: ok" in run.stdout, run.stdout
+
+
 def test_rope_zero_sizes_are_noops(ops, buf):
     p = ctypes.addressof(buf)
     lib = ops.lib()
