@@ -662,7 +662,7 @@ LEVO_OPS_API int levo_rope_qk(const levo_rope *rope, levo_stream_t stream);
  * theta of the usual schemes, written to HOST memory [rotary_dim/2]:
  *   theta[i] = base^(-2i/rotary_dim)
  *   LEVO_ROPE_SCALE_LINEAR    theta[i] / factor
- *   LEVO_ROPE_SCALE_NTK       base is taken as base * factor^(rotary_dim/(rotary_dim-2))
+ *   LEVO_ROPE_SCALE_NTK       base is taken as base * factor^(rotary_dim/(rotary_dim-2)), which must be finite
  *   LEVO_ROPE_SCALE_BY_PARTS  r = context * theta[i] / 2pi turns over the trained context,
  *                             g = clamp((r - slow) / (fast - slow), 0, 1),
  *                             (1 - g) theta[i] / factor + g theta[i]

@@ -640,6 +640,7 @@ LEVO_OPS_API int levo_rope_theta_host(double *theta_host, int64_t rotary_dim, do
     }
     const double n = static_cast<double>(rotary_dim);
     if (scaling == LEVO_ROPE_SCALE_NTK) base *= std::pow(factor, n / (n - 2.0));
+    if (!std::isfinite(base)) return fail(": the scaled base is not finite");
     for (int64_t i = 0; i < rotary_dim / 2; ++i) {
         double theta = std::pow(base, -2.0 * static_cast<double>(i) / n);
         if (scaling == LEVO_ROPE_SCALE_LINEAR) theta /= factor;

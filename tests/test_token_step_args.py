@@ -213,6 +213,15 @@ def test_theta_refuses(ops, kw, message):
         ops.rope_theta(**kw)
 
 
+@pytest.mark.parametrize("kw", [{"rotary_dim": 4, "factor": 1e200}, {"rotary_dim": 64, "base": 1e300, "factor": 1e9}])
+def test_theta_refuses_a_base_that_overflows(ops, kw):
+    """base * factor^(n / (n - 2)) beyond the range of 64 bits would give 0 for every pair but the first."""
+    with pytest.raises(ValueError, match="scaled base"):
+        ops.rope_theta(scaling="ntk", **kw)
+    large = ops.rope_theta(4, base=1e4, scaling="ntk", factor=1e150)
+    assert np.allclose(large.numpy(), [1.0, 1e-152], rtol=1e-14, atol=0)
+
+
 def sampling_args(ops, p, **changes):
     s = ops.Sampling(p, 2, 16, 16, p, None, None, None, None, 0, None, 0, 0, None, 0, 0, p, None, None, 1.0, 1.0, 0.0,
                      1.0, ops.DTYPE_F32)
