@@ -224,7 +224,9 @@ constexpr int kCtasPerSm = 3;
 // Bytes that a thread has on their way: 128 (four tokens of two 16-byte vectors).  Half and twice that cost 5 % on
 // a 4 x 2048-token prompt: fewer bytes in flight, and fewer, longer CTAs at the end.
 constexpr int kBytesInFlight = 128;
-constexpr int kMaxTurns = 4096;  // of a CTA: 32 KB of shared memory
+// Turns of a CTA's tile: 32 KB of shared memory.  (A single token that turns more than 4096 values by one value an
+// access, where a pair takes 16 bytes, has up to 64 KB to itself.)
+constexpr int kMaxTurns = 4096;
 constexpr int kMaxTile = 32;     // tokens of a CTA
 
 // A token of the tile: where its values lie (element offsets of the first head of q, k and v; out < 0: k and v have no

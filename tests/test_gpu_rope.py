@@ -390,3 +390,38 @@ def test_rope_refuses_overlapping_views(ops, dev):
     with pytest.raises(ValueError, match="another tensor's"):
         ops.rope_append_kv_t(q, q, q, theta, big[:, :6], big[:, 1:], lengths)
     assert int(torch.count_nonzero(big)) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("off,d,rot", [(0, 8192, 8192), (0, 8192, 4096), (1, 8192, 8192), (1, 8190, 54), (0, 2056, 1032),
+                                       (0, 3000, 3000)])
+def test_rope_heads_wider_than_a_block(ops, dev, dtype, interleaved, off, d, rot):
+    """More vectors in a head than a CTA has threads: the CTA goes over the head in passes, with the same turns (one
+    value an access, 8192 turned: 64 KB of them) and the same staging room."""
+    gen = torch.Generator(device=dev).manual_seed(d + rot)
+    t = DTYPES[dtype]
+    for b, s, hq, hk in ((1, 1, 1, 1), (2, 3, 2, 1)):
+        q = make(gen, (b, s, hq * d + off), t)[:, :, off:].unflatten(2, (hq, d))
+        k = make(gen, (b, s, hk * d + off), t)[:, :, off:].unflatten(2, (hk, d))
+        positions = torch.randint(0, 5000, (b, s), generator=gen, device=dev)
+        theta = ops.rope_theta(rot, device=dev)
+        check_qk(ops, q, k, theta, positions, t, interleaved=interleaved)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,dv", [(16, 8191), (64, 8192), (8192, 8), (4100, 5000)])
+def test_append_heads_wider_than_a_block(ops, dev, interleaved, d, dv):
+    gen = torch.Generator(device=dev).manual_seed(d + dv)
+    b, s, capacity, t = 2, 3, 5, torch.float16
+    q, k, v = make(gen, (b, s, 2, d), t), make(gen, (b, s, 1, d), t), make(gen, (b, s, 1, dv), t)
+    kc, vc = cache_pair(gen, b, capacity, 1, d, 1, dv, t)
+    theta = ops.rope_theta(d, device=dev)
+    lengths, counts = torch.tensor([1, 2], device=dev), torch.tensor([3, 2], device=dev)
+    positions = np.asarray([[1, 2, 3], [2, 3, 4]])
+    want_k, size, want_v = expected_caches(kc, vc, k, v, theta.cpu().numpy(), [1, 2], [3, 2], positions, interleaved)
+    qo = ops.rope_append_kv_t(q, k, v, theta, kc, vc, lengths, counts=counts, interleaved=interleaved)
+    assert_rope(kc, want_k, size, t, float(capacity), "k cache")
+    assert np.array_equal(host(vc), want_v)
+    want_q, size_q = rope(host(q), positions, theta.cpu().numpy(), interleaved)
+    assert_rope(qo, want_q, size_q, t, float(capacity), "q")
