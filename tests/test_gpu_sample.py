@@ -467,3 +467,55 @@ def test_sample_tiny_temperatures(ops, dev, rows, vocab, temperature):
     gen = torch.Generator(device=dev).manual_seed(vocab)
     for name in ("none", "k50", "k1500", "p50", "p999", "m0.1", "k+p"):
         check(ops, dev, logits, uniforms(gen, rows), temperature=temperature, **FILTERS[name])
+
+
+def plain_choice(x, u, temperature, top_k, top_p, min_p):
+    """The definition with plain F64 sums, nothing rounded to a unit: (token, log of its share, bound on the error of
+    that log), or None where a border lies so near that the documented unit may decide it."""
+    unit = 2.0 * 2.0 ** -44  # a weight's rounding to 2^-44 and the error of the exponential before it
+    order = np.argsort(-x, kind="stable")
+    if top_k:
+        order = order[:top_k]
+    v = x[order].astype(np.float64)
+    w = np.exp((v - v[0]) / temperature)
+    upto = np.cumsum(w)
+    slack = len(w) * (unit + 2.0 ** -53 * upto[-1])  # of a sum: the units', and this one's own roundings
+    keep = len(w)
+    if top_p < 1:
+        target = top_p * upto[-1]
+        if np.min(np.abs(upto - target)) <= 2 * slack:
+            return None
+        keep = max(1, int(np.sum(upto - w < target)))
+    if min_p > 0:
+        if np.min(np.abs(w - min_p)) <= unit:
+            return None
+        keep = min(keep, int(np.sum(w >= min_p)))
+    target = u * upto[keep - 1]
+    if np.min(np.abs(upto - target)) <= 2 * slack:
+        return None
+    at = min(int(np.searchsorted(upto, target, side="right")), keep - 1)
+    logprob = math.log(w[at] / upto[keep - 1])
+    return int(order[at]), logprob, 2.0 ** -24 * abs(logprob) + 2 * unit / w[at] + 2 * slack / upto[keep - 1]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["none", "k50", "k1500", "p50", "p999", "m0.1", "k+p", "all", "hot"])
+def test_sample_matches_plain_sums(ops, dev, dtype, name):
+    """Where no border lies within the weights' unit, the unit does not show."""
+    gen = torch.Generator(device=dev).manual_seed(21)
+    rows, vocab = 96, VOCAB
+    logits = (torch.linspace(0.3, 4.0, rows, device=dev)[:, None]
+              * torch.randn((rows, vocab), generator=gen, device=dev)).to(DTYPES[dtype])
+    u = uniforms(gen, rows)
+    kw = FILTERS[name]
+    tokens, logprobs, status = run(ops, logits, u, dev, **kw)
+    x, near = logits.float().cpu().numpy(), 0
+    for r in range(rows):
+        want = plain_choice(x[r], float(u[r]), float(np.float32(kw.get("temperature", 1.0))), kw.get("top_k", 0),
+                            float(np.float32(kw.get("top_p", 1.0))), float(np.float32(kw.get("min_p", 0.0))))
+        if want is None:
+            near += 1
+            continue
+        token, logprob, tol = want
+        assert tokens[r] == token and abs(logprobs[r] - logprob) <= tol, r
+    assert status == 0 and near <= rows // 8
