@@ -199,10 +199,11 @@ __device__ __forceinline__ float to_float(__nv_bfloat16 v) {
     return __bfloat162float(v);
 }
 
-// 16-byte groups whose loads a thread has on their way when it reads a row that is held: the whole of a 16384-token
-// vocabulary and of the few tokens that commonly come on top of a power of two.
-template <typename T>
-constexpr int kAheadOf = sizeof(T) == 4 ? 9 : 5;
+// 16-byte groups whose loads a thread has on their way when it reads a row that is held.  Two, four and nine of them,
+// in us from L2 (from HBM): 192 F32 rows of 16385 15.5, 15.0, 16.2 (17.4, 17.4, 20.0), 60 of 32000 24.0, 22.9, 23.5
+// (27.8, 24.9, 24.5), 192 of 8000 10.2, 10.0, 10.6; for the 16-bit types two and four: 60 rows of 32000 27.8, 27.3
+// (30.0, 30.1), 192 of 16385 11.7, 11.7 (12.7, 13.0).
+constexpr int kAhead = 4;
 
 template <typename T, bool CLUSTER, bool HELD>
 class Row {
@@ -338,7 +339,6 @@ class Row {
             f(g, v, true);
         };
         if constexpr (HELD) {
-            constexpr int kAhead = kAheadOf<T>;
             for (int g0 = begin + tid; g0 - tid < end || g0 == begin + tid; g0 += kAhead * kThreads) {
                 uint4 raw[kAhead];
 #pragma unroll
