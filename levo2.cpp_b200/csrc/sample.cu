@@ -61,11 +61,15 @@ static_assert(kList == kThreads, "a listed token a thread");
 constexpr int kMaxCluster = 8;
 constexpr int kOneShare = 32768;  // logits that a row is split from
 constexpr int kMostHeld = 32768;  // that a CTA holds: a bit each in a thread's 64
-constexpr int kRing = 8;  // groups that a thread has on their way when it reads a row again
+// Groups that a thread has on their way when it reads a row again.  Four leave room for a second CTA on the SM beside
+// the bits of 131072 edited ids; eight did not, and 128 rows of 131072 with a penalty took 153 us instead of 117 (300 of
+// 20011 72 and 56); without one the two differ by 3 % (104 and 101; 48 and 47).
+constexpr int kRing = 4;
 // Slices are at least 2^-128 of (top - v) / 2 wide, so from 15.95 T = 2^-116 down kBins of them end beyond the weights.
 constexpr float kTinyTemperature = 1e-36f;
 constexpr int kSearches = 24;  // lists of one row: three searches with up to four further cuts each, and three more
 constexpr int64_t kMaxVocab = int64_t(1) << 17;
+constexpr int kHalfAnSm = 112 * 1024;  // shared memory of a CTA that leaves room for a second one
 
 struct SampleArgs {
     const void *logits;
@@ -1288,13 +1292,15 @@ template <typename T>
 int launch_sample(SampleArgs &a, const char *what, cudaStream_t stream) {
     constexpr int L = 16 / sizeof(T);
     // A CTA's tables, its share of the row in shared memory, and whether that leaves room for a second CTA on the SM.
-    const size_t rest = 2 * kBins * sizeof(uint32_t) + 2 * kList * sizeof(u64);
+    constexpr size_t rest = 2 * kBins * sizeof(uint32_t) + 2 * kList * sizeof(u64);
+    static_assert(rest + kRing * kThreads * 16 + 2 * (kMaxVocab / 32 + 2) * sizeof(uint32_t) + sizeof(Shared) <= kHalfAnSm,
+                  "two CTAs an SM read their rows again, whatever is edited");
     auto chunk_of = [&](int ctas) { return static_cast<int>((a.vocab + ctas - 1) / ctas + 7) / 8 * 8; };
     auto slots_of = [&](int ctas) { return (chunk_of(ctas) + 2 * L + 3) / 4 * 4; };
-    auto two_an_sm = [&](int ctas) { return rest + slots_of(ctas) * sizeof(float) + sizeof(Shared) <= 112 * 1024; };
-    // One CTA a row up to kOneShare logits (three rows of 16385: one CTA each 10.8 us, two 14.0, four 13.6, since a
+    auto two_an_sm = [&](int ctas) { return rest + slots_of(ctas) * sizeof(float) + sizeof(Shared) <= kHalfAnSm; };
+    // One CTA a row up to kOneShare logits (three rows of 16385: one CTA each 10.2 us, two 13.2, four 12.6, since a
     // cluster's barriers cost more than its shorter passes save).  A longer row is split until its shares fit two an SM
-    // (5 rows of 50257: four CTAs each 28.3 us, two 33.7; one row of 131072: eight 26.5, four 40.7), as far as the SMs
+    // (5 rows of 50257: four CTAs each 27.8 us, two 32.7; one row of 131072: eight 26.8, four 37.6), as far as the SMs
     // take all CTAs at once.
     int ctas = 1;
     while (ctas < kMaxCluster && a.rows * ctas * 2 <= 2LL * sm_count() &&
@@ -1302,9 +1308,9 @@ int launch_sample(SampleArgs &a, const char *what, cudaStream_t stream) {
         ctas *= 2;
     a.chunk = chunk_of(ctas);
     a.words = a.recent || a.ignore ? (a.chunk + 31) / 32 + 2 : 0;
-    // A share that leaves room for a second CTA is held in shared memory (192 rows of 16385: 17.0 us; read again, 29),
-    // a longer one where every CTA has an SM of its own (100 rows of 20011: 18.5 us, read again 25.8; one row of 32000:
-    // 21.0 and 24.4).  Others are read again from L2 (128 rows of 131072: two CTAs a row that read again 102 us, eight
+    // A share that leaves room for a second CTA is held in shared memory (192 rows of 16385: 14.6 us; read again, 18.9),
+    // a longer one where every CTA has an SM of its own (100 rows of 20011: 18.3 us, read again 24.2; one row of 32000:
+    // 20.9 and 24.9).  Others are read again from L2 (128 rows of 131072: two CTAs a row that read again 102 us, eight
     // that hold their shares 153, four rounds of clusters).
     a.slots = slots_of(ctas);
     const bool held = two_an_sm(ctas) || (a.rows * ctas <= sm_count() && a.slots <= kMostHeld);
