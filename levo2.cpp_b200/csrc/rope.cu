@@ -255,8 +255,8 @@ __device__ __forceinline__ void copy_in(void *to, const void *from) {
 //
 // Bound by HBM on long inputs: 16001 tokens of 40 BF16 heads of 128 take 52.5 us, 6.2 TB/s (95 % of the measured copy
 // rate); 4 x 2048 tokens of 24 F16 heads 18.7 us, 5.4 TB/s (the start and end of 2048 CTAs and 220 instructions a
-// warp and 32 bytes a lane, two thirds of the issue slots); 2 x 1000 tokens of 40 F32 heads of 110, whose rows allow
-// 8 bytes an access, 16.5 us, 4.3 TB/s.  Held in registers instead of staged (two heads or tokens a thread), 4 x 2048
+// warp and 32 bytes a lane, two thirds of the issue slots); 2 x 1000 tokens of 40 F32 heads of 110, cut head by head
+// into 8 bytes an access, 16.5 us, 4.3 TB/s.  Held in registers instead of staged (two heads or tokens a thread), 4 x 2048
 // tokens took 26 to 36 us: the values on their way cost the occupancy that hides them.  One token: 3 us, the launch.
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(kMaxThreads, kCtasPerSm) rope_kernel(const RopeArgs<T> a) {

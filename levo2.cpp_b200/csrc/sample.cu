@@ -30,10 +30,11 @@
 // from L2, by a ring of cp.async copies.  Rows that are few and long are split over a cluster,
 // whose first CTA merges the histograms, takes the decisions and holds the lists.
 //
-// What bounds it: instruction issue, not bytes.  1024 rows of 16385 in F16 (half of
-// them over the whole vocabulary) take 72 us, 5.1 us of HBM time: 48 million warp
-// instructions, 62 % of the issue slots, about 35 a logit for its weight (11 of them
-// F64) and 20 for the load, the slice and the lists.  Small batches are bound by the
+// What bounds it: instruction issue, not bytes.  1024 rows of 16385 in F16 (six in ten
+// over the whole vocabulary) take 72 us, 5.1 us of HBM time: 44 million warp
+// instructions in 62 % of the issue slots, 84 a logit on the average of all rows.
+// 128 flat F32 rows of 131072, where every logit is weighed (11 F64 operations each),
+// take 101 us: 107 a logit in 59 % of the slots.  Small batches are bound by the
 // chain of some ten phases between barriers, 1 to 2 us each for a cluster.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
