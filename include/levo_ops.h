@@ -633,8 +633,8 @@ LEVO_OPS_API int levo_greedy_tokens_f32(const float *logits, int64_t rows, int64
 #define LEVO_ROPE_ADJOINT 2u
 
 /* [batch][tokens][heads][head_dim]: any layout with unit stride in head_dim.
- * A call whose outputs share an element with another tensor's output or input, or
- * with their own input but in place, is refused. */
+ * A call is refused when an output shares an element with another tensor's output or
+ * input, or, unless it is in place, with its own input. */
 typedef struct {
     const void *in;
     void *out;             /* may be `in` with the same strides (in place) */
